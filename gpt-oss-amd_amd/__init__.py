@@ -24,6 +24,11 @@ MOE_FLAG_FORCE_TILED = 4
 MOE_FLAG_FORCE_DIRECT = 8
 MOE_FLAG_FORCE_BUCKET_LAUNCH = 16
 MOE_FLAG_FUSED_GEMM_LAUNCH = 32
+MOE_ROUTE_SOFTMAX = 0
+MOE_ROUTE_SIGMOID = 1
+MOE_Q_GROUP_ROW = 0
+MOE_Q_GROUP_MX = 32
+MOE_Q_GROUP_128 = 128
 
 _c = ctypes
 _vp, _i, _ll, _f, _u, _sz = _c.c_void_p, _c.c_int, _c.c_longlong, _c.c_float, _c.c_uint, _c.c_size_t
@@ -67,6 +72,21 @@ class BlockParams(_c.Structure):
         ("flags", _c.c_uint32),
         ("next_norm_weight", _vp),
         ("next_norm_out", _vp),
+        ("route", _vp),
+    ]
+
+
+class RouteParams(_c.Structure):
+    """moe_route_params of include/moe_abi.h."""
+    _fields_ = [
+        ("struct_bytes", _c.c_uint32),
+        ("scoring", _c.c_int32),
+        ("n_groups", _c.c_int32),
+        ("groups_per_token", _c.c_int32),
+        ("group_top", _c.c_int32),
+        ("renormalize", _c.c_int32),
+        ("scale", _f),
+        ("balance_bias", _vp),
     ]
 
 
@@ -80,6 +100,12 @@ SIGNATURES = {
     "moe_gemm_router_static": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "moe_router_two_pass_scratch_bytes": (_sz, [_i, _i, _i]),
     "moe_router_two_pass_report": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "moe_route": (_i, [_vp, _vp, _vp, _i, _i, _i, _c.POINTER(RouteParams), _vp]),
+    "moe_add_rmsnorm": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _vp, _vp, _vp, _vp, _i, _vp]),
+    "moe_linear_mxfp4": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "moe_linear_int4": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "moe_int4_tiled_bytes": (None, [_i, _i, _i, _c.POINTER(_sz), _c.POINTER(_sz), _c.POINTER(_sz)]),
+    "moe_int4_repack": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "moe_topk": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
     "moe_softmax": (_i, [_vp, _i, _i, _vp]),
     "moe_bucket_by_expert": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
@@ -149,6 +175,19 @@ def _ptr(t):
     return t.data_ptr()
 
 
+def _arg(name, t, dtype, n):
+    """Address of a tensor that a kernel reads or writes n values of; None stays None."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.numel() < n:
+        raise ValueError("%s: expected %d values of %s, got %d of %s" % (name, n, dtype, t.numel(), t.dtype))
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():  # the launch goes to the current device's stream
+        raise ValueError("%s: expected a tensor on the current device" % name)
+    if not t.is_contiguous():
+        raise ValueError("%s: expected a contiguous tensor" % name)
+    return t.data_ptr()
+
+
 def _stream(stream):
     if stream is None:
         return torch.cuda.current_stream().cuda_stream
@@ -197,6 +236,31 @@ def topk(topk_values, topk_indices, router_scores, batch_size, num_experts, expe
     """src/hip/topk.hip:59."""
     _check("moe_topk", _lib.moe_topk(_ptr(topk_values), _ptr(topk_indices), _ptr(router_scores), batch_size,
                                      num_experts, experts_per_token, _stream(stream)))
+
+
+class RouteRule:
+    """A routing rule (moe_route_params): scoring "softmax" or "sigmoid", balance_bias fp32 [num_experts] on the device or None."""
+
+    def __init__(self, scoring="softmax", balance_bias=None, n_groups=1, groups_per_token=1, group_top=1, renormalize=True, scale=1.0):
+        self.balance_bias = balance_bias  # kept alive: the parameters hold its address
+        self.params = RouteParams(struct_bytes=ctypes.sizeof(RouteParams),
+                                  scoring={"softmax": MOE_ROUTE_SOFTMAX, "sigmoid": MOE_ROUTE_SIGMOID}[scoring], n_groups=n_groups,
+                                  groups_per_token=groups_per_token, group_top=group_top, renormalize=bool(renormalize), scale=scale)
+        self.ref = ctypes.byref(self.params)
+
+    def of(self, num_experts):
+        """The parameters for a call with that many experts."""
+        self.params.balance_bias = _arg("balance_bias", self.balance_bias, torch.float32, num_experts)
+        return self.ref
+
+
+def route(topk_values, topk_indices, router_logits, batch_size, num_experts, experts_per_token, rule, stream=None):
+    """Router logits [batch_size, num_experts] -> experts and weights of every token by a RouteRule (moe_route in include/moe_abi.h)."""
+    n = batch_size * experts_per_token
+    _check("moe_route",
+           _lib.moe_route(_arg("topk_values", topk_values, torch.float32, n), _arg("topk_indices", topk_indices, torch.int32, n),
+                          _arg("router_logits", router_logits, torch.float32, batch_size * num_experts), batch_size, num_experts,
+                          experts_per_token, rule.of(num_experts), _stream(stream)))
 
 
 def softmax(x, batch_size, size, stream=None):
@@ -307,6 +371,73 @@ def rmsnorm(o, x, weight, batch, size, stream=None):
     _check("moe_rmsnorm", _lib.moe_rmsnorm(_ptr(o), _ptr(x), _ptr(weight), batch, size, _stream(stream)))
 
 
+def add_rmsnorm(x_out, x, weight, batch, size, delta=None, eps=1e-5, o=None, o_bf16=None, q=None, q_scales=None, q_group=MOE_Q_GROUP_MX,
+                stream=None):
+    """x_out = x + delta and its RMSNorm as fp32 (o), bf16 (o_bf16) or e4m3 codes with scales (q, q_scales): moe_add_rmsnorm in
+    include/moe_abi.h.  q_scales: uint8 [batch, size / 32] for q_group 32, float32 [batch, ceil(size / 128)] for 128, [batch] for 0."""
+    n = batch * size
+    n_scales = batch * (1 if q_group == 0 else -(-size // q_group))
+    _check("moe_add_rmsnorm",
+           _lib.moe_add_rmsnorm(_arg("x_out", x_out, torch.float32, n), _arg("x", x, torch.float32, n), _arg("delta", delta, torch.float32, n),
+                                _arg("weight", weight, torch.bfloat16, size), batch, size, eps, _arg("o", o, torch.float32, n),
+                                _arg("o_bf16", o_bf16, torch.bfloat16, n), _arg("q", q, torch.uint8, n),
+                                _arg("q_scales", q_scales, torch.uint8 if q_group == MOE_Q_GROUP_MX else torch.float32, n_scales), q_group,
+                                _stream(stream)))
+
+
+# ---- products with 4-bit weights -----------------------------------------------------------------
+def _linear_rows(x, x_scales, B, K):
+    if x_scales is None:
+        return _arg("x", x, torch.bfloat16, B * K), None
+    return _arg("x", x, torch.uint8, B * K), _arg("x_scales", x_scales, torch.uint8, B * K // 32)
+
+
+def linear_mxfp4(y, x, tiled_blocks, tiled_scales, B, K, N, bias=None, x_scales=None, stream=None):
+    """y [B, N] = x [B, K] W^T + bias for MXFP4 weights (mxfp4_repack of one [1, N, K / 32] tensor); x bf16, or uint8 e4m3 codes with their
+    e8m0 scales [B, K / 32]: moe_linear_mxfp4 in include/moe_abi.h."""
+    xp, xs = _linear_rows(x, x_scales, B, K)
+    _check("moe_linear_mxfp4",
+           _lib.moe_linear_mxfp4(_arg("y", y, torch.float32, B * N), xp, xs, _arg("tiled_blocks", tiled_blocks, torch.uint8, N * K // 2),
+                                 _arg("tiled_scales", tiled_scales, torch.uint8, N * (-(-K // 512) * 16)),
+                                 _arg("bias", bias, torch.bfloat16, N), B, K, N, _stream(stream)))
+
+
+def int4_tiled_bytes(rows, K, group):
+    sizes = [_sz(0) for _ in range(3)]
+    _lib.moe_int4_tiled_bytes(rows, K, group, *[ctypes.byref(v) for v in sizes])
+    return tuple(v.value for v in sizes)
+
+
+def int4_repack(codes, scales, zeros=None, group=128, stream=None):
+    """codes [rows, K / 2] u8, scales [rows, ceil(K / group)] bf16, zeros [rows, ceil(K / group)] u8 or None -> what linear_int4 reads:
+    (tiled_codes, tiled_scales, tiled_zeros or None)."""
+    rows, K = codes.shape[0], 2 * codes.shape[1]
+    cb, sb, zb = int4_tiled_bytes(rows, K, group)
+    if cb == 0:
+        raise MoeError("moe_int4_tiled_bytes", -2)
+    n = rows * -(-K // group)
+    dev = codes.device
+    tc = torch.empty(cb, dtype=torch.uint8, device=dev)
+    ts = torch.empty(sb // 2, dtype=torch.bfloat16, device=dev)
+    tz = None if zeros is None else torch.empty(zb, dtype=torch.uint8, device=dev)
+    _check("moe_int4_repack",
+           _lib.moe_int4_repack(_arg("codes", codes, torch.uint8, rows * K // 2), _arg("scales", scales, torch.bfloat16, n),
+                                _arg("zeros", zeros, torch.uint8, n), rows, K, group, _ptr(tc), _ptr(ts), _ptr(tz), _stream(stream)))
+    return tc, ts, tz
+
+
+def linear_int4(y, x, tiled_codes, tiled_scales, B, K, N, group, tiled_zeros=None, bias=None, x_scales=None, stream=None):
+    """y [B, N] = x [B, K] W^T + bias for int4 weights (int4_repack): moe_linear_int4 in include/moe_abi.h; x as for linear_mxfp4."""
+    xp, xs = _linear_rows(x, x_scales, B, K)
+    rows = -(-N // 16) * 16
+    n = rows * -(-K // group) if group > 0 else 0
+    _check("moe_linear_int4",
+           _lib.moe_linear_int4(_arg("y", y, torch.float32, B * N), xp, xs,
+                                _arg("tiled_codes", tiled_codes, torch.uint8, rows * (-(-K // 128) * 64)),
+                                _arg("tiled_scales", tiled_scales, torch.bfloat16, n), _arg("tiled_zeros", tiled_zeros, torch.uint8, n),
+                                _arg("bias", bias, torch.bfloat16, N), B, K, N, group, _stream(stream)))
+
+
 # ---- MXFP4 -------------------------------------------------------------------------------------
 def dequant_mxfp4(blocks, scales, out=None, stream=None):
     """blocks [..., G, 16] u8, scales [..., G] u8 -> bf16 [..., G*32]
@@ -370,7 +501,8 @@ class MoeBlock:
     router -> top-k -> softmax -> bucketing -> experts -> combine (src/forward.cpp:317-514)."""
 
     def __init__(self, H, I, E, K, w_router, b_router, w_mlp1, b_mlp1, w_mlp2, b_mlp2, max_tokens,
-                 w_mlp1_scales=None, w_mlp2_scales=None, swiglu_limit=7.0, alpha=1.702, workspace=None):
+                 w_mlp1_scales=None, w_mlp2_scales=None, swiglu_limit=7.0, alpha=1.702, workspace=None, route=None):
+        self.route = route  # a RouteRule in place of top-k and softmax over the chosen
         self.H, self.I, self.E, self.K = H, I, E, K
         self.fmt = MOE_WEIGHTS_BF16 if w_mlp1_scales is None else MOE_WEIGHTS_MXFP4_TILED
         self.tensors = dict(w_router=w_router, b_router=b_router, w_mlp1=w_mlp1, b_mlp1=b_mlp1, w_mlp2=w_mlp2,
@@ -402,6 +534,9 @@ class MoeBlock:
         p.workspace, p.workspace_bytes = _ptr(self.workspace), self.workspace.numel()
         p.flags = flags
         p.next_norm_weight, p.next_norm_out = _ptr(next_norm_weight), _ptr(next_norm_out)
+        if self.route is not None:
+            self.route.of(self.E)
+            p.route = ctypes.addressof(self.route.params)
         return p
 
     def forward(self, t, e_agg=None, topk_i=None, topk_v=None, router_score=None, residual_x=None, flags=0,

@@ -97,7 +97,7 @@ inline bool use_fused_experts(int E, bool direct, unsigned flags) {
 }
 
 // Which kernels a block runs: block_forward_impl carries it out, moe_block_describe reports it.  The shapes are checked.
-enum class Router { kScores, kRows, kScreenRefine, kFused, kScoresFinalize, kPartialFinalize };
+enum class Router { kScores, kRows, kScreenRefine, kFused, kScoresFinalize, kPartialFinalize, kScoresRule, kPartialRule };
 struct BlockRoute {
     bool prefill, direct;
     Router router;
@@ -108,7 +108,9 @@ struct BlockRoute {
         const int fmt = p->weight_format;
         prefill = use_prefill_kernels(T, H, I, K, E, fmt, p->flags);
         direct = use_direct_bucketing(T, K, E, prefill, p->flags);
-        if (p->flags & MOE_FLAG_ROUTER_STRICT_ORDER) {
+        if (p->route) {  // the rule reads exact logits of every expert
+            router = router_scores(T, E) && !(p->flags & MOE_FLAG_ROUTER_STRICT_ORDER) ? Router::kScoresRule : Router::kPartialRule;
+        } else if (p->flags & MOE_FLAG_ROUTER_STRICT_ORDER) {
             router = Router::kPartialFinalize;
         } else if (expert_small_takes_scores(T, T * K) && use_small_kernels(T, H, I, K, E, fmt, direct, p->flags, n_cus)) {
             router = Router::kScores;  // a handful of tokens: top-k and softmax are the gate/up kernel's
@@ -139,6 +141,7 @@ struct BlockWorkspace {
     int* fused_ctr;        // counters of the one-launch expert kernel (experts_fused.hip)
     uint16_t* h_by_slot;   // [A, I] bf16 SwiGLU outputs
     float* y_by_slot;      // [A, H] fp32 down-projection rows
+    float* logits;         // [T,E] for a routing rule
     int max_tiles;
     size_t bytes;
 
@@ -166,6 +169,7 @@ struct BlockWorkspace {
         fused_ctr = static_cast<int*>(take((size_t)expert_fused_ctr_words(E) * 4));
         h_by_slot = static_cast<uint16_t*>(take(A * I * 2));
         y_by_slot = static_cast<float*>(take(A * H * 4));
+        logits = static_cast<float*>(take((size_t)T * E * 4));
         bytes = off;
     }
 };
@@ -256,6 +260,32 @@ int moe_softmax(float* x, int batch_size, int size, moe_stream_t stream) {
     if (batch_size <= 0 || size <= 0) return MOE_ERR_SHAPE;
     if (size > 64) return MOE_ERR_LIMIT;
     return launch_softmax_rows(x, batch_size, size, as_stream(stream));
+}
+
+static int check_route(const moe_route_params* rule, int E, int K) {
+    if (rule->struct_bytes != sizeof(moe_route_params)) return MOE_ERR_FORMAT;
+    if (rule->scoring != MOE_ROUTE_SOFTMAX && rule->scoring != MOE_ROUTE_SIGMOID) return MOE_ERR_FORMAT;
+    if (E <= 0 || K <= 0 || K > E) return MOE_ERR_SHAPE;
+    if (E > 1024 || K > 8 || rule->n_groups > 64) return MOE_ERR_LIMIT;
+    if (rule->n_groups <= 0 || E % rule->n_groups != 0 || rule->groups_per_token <= 0 || rule->groups_per_token > rule->n_groups)
+        return MOE_ERR_SHAPE;
+    if (rule->group_top != 1 && rule->group_top != 2) return MOE_ERR_SHAPE;
+    if (K > rule->groups_per_token * (E / rule->n_groups)) return MOE_ERR_SHAPE;
+    if ((uintptr_t)rule->balance_bias & 3u) return MOE_ERR_ALIGN;
+    return MOE_OK;
+}
+static RouteRule route_rule(const moe_route_params* r) {
+    return {r->balance_bias, r->scoring, r->n_groups, r->groups_per_token, r->group_top, r->renormalize != 0, r->scale};
+}
+
+int moe_route(float* topk_values, int* topk_indices, const float* router_logits, int batch_size, int num_experts,
+              int experts_per_token, const moe_route_params* rule, moe_stream_t stream) {
+    if (!topk_values || !topk_indices || !router_logits || !rule) return MOE_ERR_NULL;
+    if (batch_size <= 0) return MOE_ERR_SHAPE;
+    const int rc = check_route(rule, num_experts, experts_per_token);
+    if (rc) return rc;
+    return launch_route(router_logits, topk_values, topk_indices, batch_size, num_experts, experts_per_token, route_rule(rule),
+                        as_stream(stream));
 }
 
 // ---- bucketing -------------------------------------------------------------------------------
@@ -495,6 +525,75 @@ int moe_rmsnorm(float* o, const float* x, const moe_bf16_t* weight, int batch, i
     return launch_rmsnorm(o, x, weight, batch, size, as_stream(stream));
 }
 
+int moe_add_rmsnorm(float* x_out, const float* x, const float* delta, const moe_bf16_t* weight, int batch, int size, float eps,
+                    float* o, moe_bf16_t* o_bf16, uint8_t* q, void* q_scales, int q_group, moe_stream_t stream) {
+    if (!x_out || !x || !weight || (!o && !o_bf16 && !q) || (q != nullptr) != (q_scales != nullptr)) return MOE_ERR_NULL;
+    if (batch <= 0 || size <= 0 || size % 4 != 0) return MOE_ERR_SHAPE;
+    if (q && q_group != MOE_Q_GROUP_ROW && q_group != MOE_Q_GROUP_MX && q_group != MOE_Q_GROUP_128) return MOE_ERR_FORMAT;
+    if (q && q_group == MOE_Q_GROUP_MX && size % 32 != 0) return MOE_ERR_SHAPE;
+    if (((uintptr_t)x_out | (uintptr_t)x | (uintptr_t)delta | (uintptr_t)o) & 15u) return MOE_ERR_ALIGN;
+    if ((((uintptr_t)weight | (uintptr_t)o_bf16) & 7u) || ((uintptr_t)q & 3u)) return MOE_ERR_ALIGN;
+    if (q && q_group != MOE_Q_GROUP_MX && ((uintptr_t)q_scales & 3u)) return MOE_ERR_ALIGN;
+    return launch_add_rmsnorm({x_out, x, delta, weight, o, o_bf16, q, static_cast<uint8_t*>(q_scales), q_group, size, eps}, batch,
+                              as_stream(stream));
+}
+
+// ---- products with 4-bit weights ---------------------------------------------------------------
+static int check_linear(const void* y, const void* x, const void* w, const void* w_scales, const void* bias, int B, int K, int N) {
+    if (!y || !x || !w || !w_scales) return MOE_ERR_NULL;
+    if (B <= 0 || K <= 0 || N <= 0 || K % 32 != 0) return MOE_ERR_SHAPE;
+    if (B > 65535) return MOE_ERR_LIMIT;
+    if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)w_scales) & 15u) return MOE_ERR_ALIGN;
+    if (((uintptr_t)y & 3u) || ((uintptr_t)bias & 1u)) return MOE_ERR_ALIGN;
+    return MOE_OK;
+}
+
+int moe_linear_mxfp4(float* y, const void* x, const uint8_t* x_scales, const uint8_t* tiled_blocks, const uint8_t* tiled_scales,
+                     const moe_bf16_t* bias, int B, int K, int N, moe_stream_t stream) {
+    const int rc = check_linear(y, x, tiled_blocks, tiled_scales, bias, B, K, N);
+    if (rc) return rc;
+    if (N % 64 != 0) return MOE_ERR_SHAPE;
+    return launch_linear_w4({y, x, x_scales, tiled_blocks, tiled_scales, nullptr, bias, B, K, N}, 0, as_stream(stream));
+}
+
+int moe_linear_int4(float* y, const void* x, const uint8_t* x_scales, const uint8_t* tiled_codes, const moe_bf16_t* tiled_scales,
+                    const uint8_t* tiled_zeros, const moe_bf16_t* bias, int B, int K, int N, int group, moe_stream_t stream) {
+    const int rc = check_linear(y, x, tiled_codes, tiled_scales, bias, B, K, N);
+    if (rc) return rc;
+    if (group != 32 && group != 64 && group != 128) return MOE_ERR_FORMAT;
+    if ((uintptr_t)tiled_zeros & 15u) return MOE_ERR_ALIGN;
+    return launch_linear_w4({y, x, x_scales, tiled_codes, reinterpret_cast<const uint8_t*>(tiled_scales), tiled_zeros, bias, B, K, N}, group,
+                            as_stream(stream));
+}
+
+// the repack's grids count 256 lanes, and scales, to a block
+static int check_int4(int rows, int K, int group) {
+    if (rows <= 0 || K <= 0 || K % 32 != 0) return MOE_ERR_SHAPE;
+    if (group != 32 && group != 64 && group != 128) return MOE_ERR_FORMAT;
+    if ((long long)ceil_div(rows, 16) * ceil_div(K, 32) * 16 > 0x7FFFFFFFll * 256) return MOE_ERR_LIMIT;
+    return MOE_OK;
+}
+
+void moe_int4_tiled_bytes(int rows, int K, int group, size_t* code_bytes, size_t* scale_bytes, size_t* zero_bytes) {
+    if (check_int4(rows, K, group) != MOE_OK) {
+        if (code_bytes) *code_bytes = 0;
+        if (scale_bytes) *scale_bytes = 0;
+        if (zero_bytes) *zero_bytes = 0;
+        return;
+    }
+    int4_tiled_bytes(rows, K, group, code_bytes, scale_bytes, zero_bytes);
+}
+
+int moe_int4_repack(const uint8_t* codes, const moe_bf16_t* scales, const uint8_t* zeros, int rows, int K, int group,
+                    uint8_t* tiled_codes, moe_bf16_t* tiled_scales, uint8_t* tiled_zeros, moe_stream_t stream) {
+    if (!codes || !scales || !tiled_codes || !tiled_scales || (zeros && !tiled_zeros)) return MOE_ERR_NULL;
+    const int rc = check_int4(rows, K, group);
+    if (rc) return rc;
+    if (((uintptr_t)codes & 3u) || ((uintptr_t)scales & 1u)) return MOE_ERR_ALIGN;
+    if (((uintptr_t)tiled_codes | (uintptr_t)tiled_scales | (uintptr_t)tiled_zeros) & 15u) return MOE_ERR_ALIGN;
+    return launch_int4_repack(codes, scales, zeros, rows, K, group, tiled_codes, tiled_scales, tiled_zeros, as_stream(stream));
+}
+
 // ---- MXFP4 -----------------------------------------------------------------------------------
 int moe_dequant_mxfp4(const uint8_t* blocks, const uint8_t* scales, long long n_blocks, moe_bf16_t* out,
                       moe_stream_t stream) {
@@ -713,21 +812,31 @@ struct ExpertPlan {
     }
 };
 
-static int block_forward_impl(const moe_block_params* caller, moe_stream_t stream_, moe_stage_timer* timer) {
+// The caller's parameter block in today's struct: the structs as they were before next_norm_weight / next_norm_out and before route were
+// appended are still accepted, and what they lack is NULL.
+static int read_block_params(const moe_block_params* caller, moe_block_params* p) {
     if (!caller) return MOE_ERR_NULL;
-    // the struct as it was before next_norm_weight / next_norm_out were appended is still accepted
-    constexpr size_t kOldBytes = offsetof(moe_block_params, next_norm_weight);
-    if (caller->struct_bytes != sizeof(moe_block_params) && caller->struct_bytes != kOldBytes) return MOE_ERR_FORMAT;
-    moe_block_params local{};
-    memcpy(&local, caller, caller->struct_bytes);
+    if (caller->struct_bytes != sizeof(moe_block_params) && caller->struct_bytes != offsetof(moe_block_params, route) &&
+        caller->struct_bytes != offsetof(moe_block_params, next_norm_weight))
+        return MOE_ERR_FORMAT;
+    memset(p, 0, sizeof(*p));
+    memcpy(p, caller, caller->struct_bytes);
+    return MOE_OK;
+}
+
+static int block_forward_impl(const moe_block_params* caller, moe_stream_t stream_, moe_stage_timer* timer) {
+    moe_block_params local;
+    int rc = read_block_params(caller, &local);
+    if (rc) return rc;
     const moe_block_params* p = &local;
     if ((p->next_norm_weight != nullptr) != (p->next_norm_out != nullptr)) return MOE_ERR_NULL;
     if (p->next_norm_out && !p->residual_x) return MOE_ERR_NULL;
     if (((uintptr_t)p->next_norm_out & 15u) || ((uintptr_t)p->next_norm_weight & 7u)) return MOE_ERR_ALIGN;
     const int T = p->n_tokens, H = p->hidden_dim, I = p->intermediate_dim, E = p->n_experts,
               K = p->experts_per_token;
-    int rc = check_dims(T, H, I, E, K);
+    rc = check_dims(T, H, I, E, K);
     if (rc) return rc;
+    if (p->route && (rc = check_route(p->route, E, K))) return rc;
     if (!p->t || !p->w_router || !p->b_router || !p->w_mlp1 || !p->b_mlp1 || !p->w_mlp2 || !p->b_mlp2 ||
         !p->e_agg || !p->topk_i || !p->topk_v)
         return MOE_ERR_NULL;
@@ -780,6 +889,23 @@ static int block_forward_impl(const moe_block_params* caller, moe_stream_t strea
             if ((rc = mark())) return rc;
             rc = launch_router_finalize(ws.router_partial, S, nullptr, p->b_router, p->router_score, p->topk_v, p->topk_i, T,
                                         E, K, 1, 1, stream);
+            break;
+        }
+        case Router::kScoresRule:
+        case Router::kPartialRule: {
+            float* const logits = p->router_score ? p->router_score : ws.logits;
+            if (route.router == Router::kScoresRule) {
+                rc = launch_router_scores(p->t, p->w_router, p->b_router, ws.t_bf16, logits, T, H, E, stream);
+            } else {
+                const int S = router_segments(T, E, H, (p->flags & MOE_FLAG_ROUTER_STRICT_ORDER) != 0);
+                rc = launch_router_partial(p->t, p->w_router, ws.router_partial, ws.t_bf16, T, H, E, S, stream);
+                if (!rc)
+                    rc = launch_router_finalize(ws.router_partial, S, nullptr, p->b_router, logits, nullptr, nullptr, T, E, 0, 0, 0,
+                                                stream);
+            }
+            if (rc) return rc;
+            if ((rc = mark())) return rc;
+            rc = launch_route(logits, p->topk_v, p->topk_i, T, E, K, route_rule(p->route), stream);
             break;
         }
     }
@@ -873,14 +999,13 @@ int moe_block_forward_layers(const moe_block_params* params, int n_layers, moe_s
 int moe_block_describe(const moe_block_params* caller, char* text, size_t text_bytes) {
     if (!caller || !text) return MOE_ERR_NULL;
     if (text_bytes < 64) return MOE_ERR_LIMIT;
-    constexpr size_t kOldBytes = offsetof(moe_block_params, next_norm_weight);
-    if (caller->struct_bytes != sizeof(moe_block_params) && caller->struct_bytes != kOldBytes) return MOE_ERR_FORMAT;
-    moe_block_params local{};
-    memcpy(&local, caller, caller->struct_bytes);
+    moe_block_params local;
+    int rc = read_block_params(caller, &local);
+    if (rc) return rc;
     const moe_block_params* p = &local;
     const int T = p->n_tokens, H = p->hidden_dim, I = p->intermediate_dim, E = p->n_experts,
               K = p->experts_per_token;
-    int rc = check_dims(T, H, I, E, K);
+    rc = check_dims(T, H, I, E, K);
     if (rc) return rc;
     const int fmt = p->weight_format;
     if (fmt != MOE_WEIGHTS_BF16 && fmt != MOE_WEIGHTS_MXFP4_TILED) return MOE_ERR_FORMAT;
@@ -894,6 +1019,8 @@ int moe_block_describe(const moe_block_params* caller, char* text, size_t text_b
         case Router::kFused: router = "router_fused_kernel"; break;
         case Router::kScoresFinalize: router = "router_scores_kernel + router_finalize_kernel"; break;
         case Router::kPartialFinalize: router = "router_partial_kernel + router_finalize_kernel"; break;
+        case Router::kScoresRule: router = "router_scores_kernel + route_kernel"; break;
+        case Router::kPartialRule: router = "router_partial_kernel + router_finalize_kernel + route_kernel"; break;
     }
     const int tile_tokens = tile_tokens_of(prefill, fmt);
     BlockWorkspace ws(nullptr, T, H, I, E, K);
@@ -947,15 +1074,13 @@ void moe_synth_normal_table(float* h_table) {
 int moe_block_down_gemm(const moe_block_params* caller, const moe_bf16_t* h_by_assignment, float* y_by_assignment,
                         moe_stream_t stream_) {
     if (!caller || !h_by_assignment || !y_by_assignment) return MOE_ERR_NULL;
-    // as moe_block_forward: the struct as it was before next_norm_weight / next_norm_out is still accepted
-    constexpr size_t kOldBytes = offsetof(moe_block_params, next_norm_weight);
-    if (caller->struct_bytes != sizeof(moe_block_params) && caller->struct_bytes != kOldBytes) return MOE_ERR_FORMAT;
-    moe_block_params local{};
-    memcpy(&local, caller, caller->struct_bytes);
+    moe_block_params local;
+    int rc = read_block_params(caller, &local);
+    if (rc) return rc;
     const moe_block_params* p = &local;
     const int T = p->n_tokens, H = p->hidden_dim, I = p->intermediate_dim, E = p->n_experts,
               K = p->experts_per_token;
-    int rc = check_dims(T, H, I, E, K);
+    rc = check_dims(T, H, I, E, K);
     if (rc) return rc;
     if (!p->w_mlp2 || !p->b_mlp2 || !p->topk_i || !p->topk_v) return MOE_ERR_NULL;
     const int fmt = p->weight_format;

@@ -41,6 +41,14 @@ int launch_router_two_pass(const float* x, const uint16_t* w, const uint16_t* bi
                            hipStream_t stream, hipEvent_t between, float* approx_out = nullptr,
                            float* delta_out = nullptr, int* n_cand_out = nullptr);
 
+// ---- route.hip --------------------------------------------------------------------------------
+struct RouteRule {  // moe_route_params
+    const float* bias;
+    int scoring, n_groups, groups_per_token, group_top, renormalize;
+    float scale;
+};
+int launch_route(const float* logits, float* topk_v, int* topk_i, int T, int E, int K, const RouteRule& rule, hipStream_t stream);
+
 // ---- bucket.hip -------------------------------------------------------------------------------
 // Token-block map consumed by the expert kernels: tile i covers rows
 // [tile_row0[i], tile_row0[i] + tile_rows[i]) of tokens_flat, all routed to tile_expert[i].
@@ -165,6 +173,38 @@ int launch_combine_norm(const float* y_by_slot, const int* slot_of, const int* t
                         int H, hipStream_t stream);
 int launch_vecadd_and_zero(float* a, float* b, float weight, int batch, int size, hipStream_t stream);
 int launch_rmsnorm(float* o, const float* x, const uint16_t* weight, int batch, int size, hipStream_t stream);
+
+// ---- add_norm.hip ------------------------------------------------------------------------------
+struct AddNormArgs {
+    float* x_out;
+    const float* x;
+    const float* delta;      // or nullptr
+    const uint16_t* weight;  // bf16
+    float* o;                // or nullptr
+    uint16_t* o_bf16;        // or nullptr
+    uint8_t* q;              // or nullptr
+    uint8_t* q_scales;
+    int q_group;             // 32 (e8m0 scales), 128 (fp32) or 0 (fp32, one a row)
+    int size;
+    float eps;
+};
+int launch_add_rmsnorm(const AddNormArgs& a, int batch, hipStream_t stream);
+
+// ---- linear_w4.hip -----------------------------------------------------------------------------
+struct LinearArgs {
+    float* y;                 // [B, N]
+    const void* x;            // [B, K] bf16, or e4m3 with x_scales
+    const uint8_t* x_scales;  // [B, K / 32] e8m0, or nullptr
+    const uint8_t* w;         // tiled
+    const uint8_t* w_scales;
+    const uint8_t* w_zeros;   // int4: or nullptr (8 everywhere)
+    const uint16_t* bias;     // bf16 [N], or nullptr
+    int B, K, N;
+};
+int launch_linear_w4(const LinearArgs& a, int group, hipStream_t stream);  // group: 0 MXFP4, else of the int4 scales
+void int4_tiled_bytes(int rows, int K, int group, size_t* codes, size_t* scales, size_t* zeros);
+int launch_int4_repack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int rows, int K, int group, uint8_t* tiled_codes,
+                       uint16_t* tiled_scales, uint8_t* tiled_zeros, hipStream_t stream);
 
 // ---- mxfp4.hip ---------------------------------------------------------------------------------
 void mxfp4_tiled_bytes(int rows, int K, size_t* block_bytes, size_t* scale_bytes);

@@ -121,6 +121,32 @@ MOE_API int moe_topk(float* topk_values, int* topk_indices, const float* router_
  * size <= 64. */
 MOE_API int moe_softmax(float* x, int batch_size, int size, moe_stream_t stream);
 
+/* Routing by score: router logits -> topk_values / topk_indices [batch_size, experts_per_token], for models whose rule is not
+ * "softmax over the largest logits" (moe_topk + moe_softmax).  No counterpart in the reference.  Per token, with l its logits:
+ *   score[e]  = 1 / (1 + exp(-l[e]))  or  exp(l[e] - max l) / sum exp(l - max l), computed in fp64 and rounded to fp32; a logit of
+ *               -infinity scores 0 (so does a token's every expert if all its logits are)
+ *   choice[e] = score[e] + balance_bias[e]  (fp32; score[e] without a bias)
+ *   groups    : experts form n_groups runs of num_experts / n_groups; a group's value is the sum (fp32) of its group_top largest choices
+ *               (group_top 1 or 2; a group of one expert has one); the groups_per_token groups of largest value stay, equal ones: the lower
+ *   chosen    : the experts_per_token largest choices of the groups that stay, in descending order, equal ones: the lower index.  A NaN
+ *               counts as larger than any number.  The indices of a token are distinct and in range whatever its logits hold
+ *   value     = score[chosen], divided by the sum over the chosen if renormalize (0 where that sum is 0), times scale (fp64, rounded once)
+ * num_experts <= 1024, a multiple of n_groups; n_groups <= 64; experts_per_token <= 8 and <= the experts of the groups that stay.  The
+ * rule is host memory, read during the call; balance_bias [num_experts] is device memory or NULL. */
+enum { MOE_ROUTE_SOFTMAX = 0, MOE_ROUTE_SIGMOID = 1 };
+typedef struct moe_route_params {
+    uint32_t struct_bytes;    /* sizeof(moe_route_params) of the caller's header */
+    int32_t scoring;          /* MOE_ROUTE_* */
+    int32_t n_groups;         /* 1: no groups */
+    int32_t groups_per_token;
+    int32_t group_top;        /* 1 or 2 */
+    int32_t renormalize;
+    float scale;
+    const float* balance_bias;
+} moe_route_params;
+MOE_API int moe_route(float* topk_values, int* topk_indices, const float* router_logits, int batch_size, int num_experts,
+                      int experts_per_token, const moe_route_params* rule, moe_stream_t stream);
+
 /* ------------------------------------------------------------------------------------------
  * Expert token bucketing
  * ---------------------------------------------------------------------------------------- */
@@ -250,6 +276,50 @@ MOE_API int moe_vecadd_and_zero(float* a, float* b, float weight, int batch, int
 MOE_API int moe_rmsnorm(float* o, const float* x, const moe_bf16_t* weight, int batch, int size,
                 moe_stream_t stream);
 
+/* Residual add, RMSNorm and its result in the type that the next product reads (no counterpart in the reference, whose products read
+ * fp32 rows):
+ *   x_out = x + delta (fp32; x without a delta),  y = RMSNorm(x_out) with the arithmetic of moe_rmsnorm and the caller's eps
+ * and of y what is asked for, at least one: o [batch, size] fp32; o_bf16 [batch, size] (round to nearest even); q [batch, size] e4m3 codes
+ * with q_scales, value = code * scale:
+ *   q_group 32   e8m0 bytes [batch, size / 32]: the smallest power of two, from 2^-126, that leaves the largest |y| of the 32 at 448 or
+ *                below (byte b stands for 2^(b - 127)); size % 32 == 0.  What moe_linear_mxfp4 and moe_linear_int4 take as x, x_scales
+ *   q_group 128  fp32 [batch, ceil(size / 128)], the last group may be shorter;  q_group 0  fp32 [batch], one a row:
+ *                a = max(largest |y|, 2^-100), scale = a / 448, code = e4m3(y * (448 / a))
+ * Codes are rounded to nearest even.  A group that holds an infinity or a NaN has a NaN for its scale and for every code.  x_out may be x;
+ * otherwise no output may overlap an input.  size % 4 == 0; x, x_out, delta and o 16-byte aligned, weight and o_bf16 8-byte, q and fp32 scales
+ * 4-byte. */
+enum { MOE_Q_GROUP_ROW = 0, MOE_Q_GROUP_MX = 32, MOE_Q_GROUP_128 = 128 };
+MOE_API int moe_add_rmsnorm(float* x_out, const float* x, const float* delta, const moe_bf16_t* weight, int batch, int size, float eps,
+                            float* o, moe_bf16_t* o_bf16, uint8_t* q, void* q_scales, int q_group, moe_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Products of a few rows with 4-bit weights (the dense counterpart of the expert products; none in the reference,
+ * which holds all its weights in bf16)
+ * ---------------------------------------------------------------------------------------- */
+
+/* y[b, n] = bias[n] + sum_k x[b, k] W[n, k], fp32 sums, for B rows and an N x K matrix; made for decode-sized batches (the weights are read
+ * once per 64 rows).  x [B, K] is bf16 (x_scales NULL) or e4m3 codes with x_scales [B, K / 32] e8m0 as moe_add_rmsnorm writes them (byte 0
+ * counts as a factor of 0, as in weights).  bias [N] bf16 or NULL.  K % 32 == 0, B <= 65535; x and the tiled tensors 16-byte aligned.
+ * Deterministic, and a row's result does not depend on the rows around it.
+ *
+ * moe_linear_mxfp4: tiled_blocks / tiled_scales of moe_mxfp4_repack(E = 1, rows = N, K); N % 64 == 0.
+ *
+ * moe_linear_int4: W[n, k] = (code - zero) * scale, codes 0..15, one bf16 scale and one zero point 0..15 for every `group` (32, 64 or 128) values of a
+ * row, the last group of which may be shorter; any N.  tiled_* come from moe_int4_repack; tiled_zeros NULL: zero points of 8.  A row of
+ * x with an infinity or a NaN may give NaN where exact arithmetic gives an infinity. */
+MOE_API int moe_linear_mxfp4(float* y, const void* x, const uint8_t* x_scales, const uint8_t* tiled_blocks, const uint8_t* tiled_scales,
+                             const moe_bf16_t* bias, int B, int K, int N, moe_stream_t stream);
+MOE_API int moe_linear_int4(float* y, const void* x, const uint8_t* x_scales, const uint8_t* tiled_codes, const moe_bf16_t* tiled_scales,
+                            const uint8_t* tiled_zeros, const moe_bf16_t* bias, int B, int K, int N, int group, moe_stream_t stream);
+
+/* Load-time repack of an int4 matrix: codes [rows, K / 2] u8 (low half of a byte = even element), scales [rows, ceil(K / group)] bf16, zeros
+ * [rows, ceil(K / group)] u8 (low four bits) or NULL (then tiled_zeros is not written and may be NULL) -> the layout moe_linear_int4 reads.
+ * moe_int4_tiled_bytes gives the three destination sizes (0 for sizes that the repack rejects).  K % 32 == 0; codes 4-byte aligned, tiled
+ * tensors 16-byte. */
+MOE_API void moe_int4_tiled_bytes(int rows, int K, int group, size_t* code_bytes, size_t* scale_bytes, size_t* zero_bytes);
+MOE_API int moe_int4_repack(const uint8_t* codes, const moe_bf16_t* scales, const uint8_t* zeros, int rows, int K, int group,
+                            uint8_t* tiled_codes, moe_bf16_t* tiled_scales, uint8_t* tiled_zeros, moe_stream_t stream);
+
 /* ------------------------------------------------------------------------------------------
  * MXFP4 (no counterpart at run time in the reference, which dequantises offline:
  * tools/model_export/gpt-oss-20b/export_model_bin.py:95-133)
@@ -322,6 +392,10 @@ typedef struct moe_block_params {
      * the behaviour of NULL. */
     const moe_bf16_t* next_norm_weight; /* [H] */
     float* next_norm_out;               /* [B,H] */
+    /* Optional: the routing rule (host memory, read during the call) in place of top-k and softmax over the chosen, applied to the router's
+     * logits (exact ones, as moe_gemm_router).  topk_i / topk_v are then what moe_route gives.  A caller built against the struct
+     * without this member gets the behaviour of NULL. */
+    const moe_route_params* route;
 } moe_block_params;
 
 enum {
