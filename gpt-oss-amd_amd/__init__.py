@@ -31,6 +31,7 @@ MOE_Q_GROUP_MX = 32
 MOE_Q_GROUP_128 = 128
 
 _c = ctypes
+_f32, _bf16, _u8 = torch.float32, torch.bfloat16, torch.uint8
 _vp, _i, _ll, _f, _u, _sz = _c.c_void_p, _c.c_int, _c.c_longlong, _c.c_float, _c.c_uint, _c.c_size_t
 
 
@@ -175,22 +176,31 @@ def _ptr(t):
     return t.data_ptr()
 
 
-def _arg(name, t, dtype, n):
-    """Address of a tensor that a kernel reads or writes n values of; None stays None."""
+def _device():
+    """Index of the current device; without one an index that no tensor has."""
+    try:
+        return torch._C._cuda_getDevice()
+    except RuntimeError:
+        return -2
+
+
+def _arg(name, t, dtype, n, dev):
+    """Address of a contiguous tensor on device `dev`, the current one, that a kernel reads or writes n values of; None stays None."""
     if t is None:
         return None
     if t.dtype is not dtype or t.numel() < n:
         raise ValueError("%s: expected %d values of %s, got %d of %s" % (name, n, dtype, t.numel(), t.dtype))
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():  # the launch goes to the current device's stream
+    if t.get_device() != dev:  # the launch goes to the current device's stream
         raise ValueError("%s: expected a tensor on the current device" % name)
     if not t.is_contiguous():
         raise ValueError("%s: expected a contiguous tensor" % name)
     return t.data_ptr()
 
 
+# torch.cuda.current_stream() makes a stream object on every call: 2.9 us, as much as a launch; the handle alone 0.2
 def _stream(stream):
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
 
 
@@ -250,17 +260,18 @@ class RouteRule:
 
     def of(self, num_experts):
         """The parameters for a call with that many experts."""
-        self.params.balance_bias = _arg("balance_bias", self.balance_bias, torch.float32, num_experts)
+        self.params.balance_bias = _arg("balance_bias", self.balance_bias, torch.float32, num_experts, _device())
         return self.ref
 
 
 def route(topk_values, topk_indices, router_logits, batch_size, num_experts, experts_per_token, rule, stream=None):
     """Router logits [batch_size, num_experts] -> experts and weights of every token by a RouteRule (moe_route in include/moe_abi.h)."""
-    n = batch_size * experts_per_token
-    _check("moe_route",
-           _lib.moe_route(_arg("topk_values", topk_values, torch.float32, n), _arg("topk_indices", topk_indices, torch.int32, n),
-                          _arg("router_logits", router_logits, torch.float32, batch_size * num_experts), batch_size, num_experts,
-                          experts_per_token, rule.of(num_experts), _stream(stream)))
+    n, dev = batch_size * experts_per_token, _device()
+    rc = _lib.moe_route(_arg("topk_values", topk_values, _f32, n, dev), _arg("topk_indices", topk_indices, torch.int32, n, dev),
+                        _arg("router_logits", router_logits, _f32, batch_size * num_experts, dev), batch_size, num_experts,
+                        experts_per_token, rule.of(num_experts), _stream(stream))
+    if rc:
+        raise MoeError("moe_route", rc)
 
 
 def softmax(x, batch_size, size, stream=None):
@@ -375,31 +386,33 @@ def add_rmsnorm(x_out, x, weight, batch, size, delta=None, eps=1e-5, o=None, o_b
                 stream=None):
     """x_out = x + delta and its RMSNorm as fp32 (o), bf16 (o_bf16) or e4m3 codes with scales (q, q_scales): moe_add_rmsnorm in
     include/moe_abi.h.  q_scales: uint8 [batch, size / 32] for q_group 32, float32 [batch, ceil(size / 128)] for 128, [batch] for 0."""
-    n = batch * size
+    n, dev = batch * size, _device()
     n_scales = batch * (1 if q_group == 0 else -(-size // q_group))
-    _check("moe_add_rmsnorm",
-           _lib.moe_add_rmsnorm(_arg("x_out", x_out, torch.float32, n), _arg("x", x, torch.float32, n), _arg("delta", delta, torch.float32, n),
-                                _arg("weight", weight, torch.bfloat16, size), batch, size, eps, _arg("o", o, torch.float32, n),
-                                _arg("o_bf16", o_bf16, torch.bfloat16, n), _arg("q", q, torch.uint8, n),
-                                _arg("q_scales", q_scales, torch.uint8 if q_group == MOE_Q_GROUP_MX else torch.float32, n_scales), q_group,
-                                _stream(stream)))
+    rc = _lib.moe_add_rmsnorm(_arg("x_out", x_out, _f32, n, dev), _arg("x", x, _f32, n, dev), _arg("delta", delta, _f32, n, dev),
+                              _arg("weight", weight, _bf16, size, dev), batch, size, eps, _arg("o", o, _f32, n, dev),
+                              _arg("o_bf16", o_bf16, _bf16, n, dev), _arg("q", q, _u8, n, dev),
+                              _arg("q_scales", q_scales, _u8 if q_group == MOE_Q_GROUP_MX else _f32, n_scales, dev), q_group, _stream(stream))
+    if rc:
+        raise MoeError("moe_add_rmsnorm", rc)
 
 
 # ---- products with 4-bit weights -----------------------------------------------------------------
-def _linear_rows(x, x_scales, B, K):
+def _linear_rows(x, x_scales, B, K, dev):
     if x_scales is None:
-        return _arg("x", x, torch.bfloat16, B * K), None
-    return _arg("x", x, torch.uint8, B * K), _arg("x_scales", x_scales, torch.uint8, B * K // 32)
+        return _arg("x", x, _bf16, B * K, dev), None
+    return _arg("x", x, _u8, B * K, dev), _arg("x_scales", x_scales, _u8, B * K // 32, dev)
 
 
 def linear_mxfp4(y, x, tiled_blocks, tiled_scales, B, K, N, bias=None, x_scales=None, stream=None):
     """y [B, N] = x [B, K] W^T + bias for MXFP4 weights (mxfp4_repack of one [1, N, K / 32] tensor); x bf16, or uint8 e4m3 codes with their
     e8m0 scales [B, K / 32]: moe_linear_mxfp4 in include/moe_abi.h."""
-    xp, xs = _linear_rows(x, x_scales, B, K)
-    _check("moe_linear_mxfp4",
-           _lib.moe_linear_mxfp4(_arg("y", y, torch.float32, B * N), xp, xs, _arg("tiled_blocks", tiled_blocks, torch.uint8, N * K // 2),
-                                 _arg("tiled_scales", tiled_scales, torch.uint8, N * (-(-K // 512) * 16)),
-                                 _arg("bias", bias, torch.bfloat16, N), B, K, N, _stream(stream)))
+    dev = _device()
+    xp, xs = _linear_rows(x, x_scales, B, K, dev)
+    rc = _lib.moe_linear_mxfp4(_arg("y", y, _f32, B * N, dev), xp, xs, _arg("tiled_blocks", tiled_blocks, _u8, N * K // 2, dev),
+                               _arg("tiled_scales", tiled_scales, _u8, N * (-(-K // 512) * 16), dev), _arg("bias", bias, _bf16, N, dev),
+                               B, K, N, _stream(stream))
+    if rc:
+        raise MoeError("moe_linear_mxfp4", rc)
 
 
 def int4_tiled_bytes(rows, K, group):
@@ -416,26 +429,27 @@ def int4_repack(codes, scales, zeros=None, group=128, stream=None):
     if cb == 0:
         raise MoeError("moe_int4_tiled_bytes", -2)
     n = rows * -(-K // group)
-    dev = codes.device
+    dev, index = codes.device, _device()
     tc = torch.empty(cb, dtype=torch.uint8, device=dev)
     ts = torch.empty(sb // 2, dtype=torch.bfloat16, device=dev)
     tz = None if zeros is None else torch.empty(zb, dtype=torch.uint8, device=dev)
     _check("moe_int4_repack",
-           _lib.moe_int4_repack(_arg("codes", codes, torch.uint8, rows * K // 2), _arg("scales", scales, torch.bfloat16, n),
-                                _arg("zeros", zeros, torch.uint8, n), rows, K, group, _ptr(tc), _ptr(ts), _ptr(tz), _stream(stream)))
+           _lib.moe_int4_repack(_arg("codes", codes, _u8, rows * K // 2, index), _arg("scales", scales, _bf16, n, index),
+                                _arg("zeros", zeros, _u8, n, index), rows, K, group, _ptr(tc), _ptr(ts), _ptr(tz), _stream(stream)))
     return tc, ts, tz
 
 
 def linear_int4(y, x, tiled_codes, tiled_scales, B, K, N, group, tiled_zeros=None, bias=None, x_scales=None, stream=None):
     """y [B, N] = x [B, K] W^T + bias for int4 weights (int4_repack): moe_linear_int4 in include/moe_abi.h; x as for linear_mxfp4."""
-    xp, xs = _linear_rows(x, x_scales, B, K)
+    dev = _device()
+    xp, xs = _linear_rows(x, x_scales, B, K, dev)
     rows = -(-N // 16) * 16
-    n = rows * -(-K // group) if group > 0 else 0
-    _check("moe_linear_int4",
-           _lib.moe_linear_int4(_arg("y", y, torch.float32, B * N), xp, xs,
-                                _arg("tiled_codes", tiled_codes, torch.uint8, rows * (-(-K // 128) * 64)),
-                                _arg("tiled_scales", tiled_scales, torch.bfloat16, n), _arg("tiled_zeros", tiled_zeros, torch.uint8, n),
-                                _arg("bias", bias, torch.bfloat16, N), B, K, N, group, _stream(stream)))
+    n = rows * (-(-K // 256) * 256 // group) if group > 0 else 0
+    rc = _lib.moe_linear_int4(_arg("y", y, _f32, B * N, dev), xp, xs, _arg("tiled_codes", tiled_codes, _u8, rows * (-(-K // 128) * 64), dev),
+                              _arg("tiled_scales", tiled_scales, _bf16, n, dev), _arg("tiled_zeros", tiled_zeros, _u8, n, dev),
+                              _arg("bias", bias, _bf16, N, dev), B, K, N, group, _stream(stream))
+    if rc:
+        raise MoeError("moe_linear_int4", rc)
 
 
 # ---- MXFP4 -------------------------------------------------------------------------------------

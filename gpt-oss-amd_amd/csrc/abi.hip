@@ -542,7 +542,7 @@ int moe_add_rmsnorm(float* x_out, const float* x, const float* delta, const moe_
 static int check_linear(const void* y, const void* x, const void* w, const void* w_scales, const void* bias, int B, int K, int N) {
     if (!y || !x || !w || !w_scales) return MOE_ERR_NULL;
     if (B <= 0 || K <= 0 || N <= 0 || K % 32 != 0) return MOE_ERR_SHAPE;
-    if (B > 65535) return MOE_ERR_LIMIT;
+    if (B > 65535 || K > (1 << 24)) return MOE_ERR_LIMIT;
     if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)w_scales) & 15u) return MOE_ERR_ALIGN;
     if (((uintptr_t)y & 3u) || ((uintptr_t)bias & 1u)) return MOE_ERR_ALIGN;
     return MOE_OK;
@@ -553,7 +553,8 @@ int moe_linear_mxfp4(float* y, const void* x, const uint8_t* x_scales, const uin
     const int rc = check_linear(y, x, tiled_blocks, tiled_scales, bias, B, K, N);
     if (rc) return rc;
     if (N % 64 != 0) return MOE_ERR_SHAPE;
-    return launch_linear_w4({y, x, x_scales, tiled_blocks, tiled_scales, nullptr, bias, B, K, N}, 0, as_stream(stream));
+    return launch_linear_w4({y, x, x_scales, tiled_blocks, tiled_scales, nullptr, bias, B, K, N, 0}, 0, device_cu_count(),
+                            as_stream(stream));
 }
 
 int moe_linear_int4(float* y, const void* x, const uint8_t* x_scales, const uint8_t* tiled_codes, const moe_bf16_t* tiled_scales,
@@ -562,8 +563,8 @@ int moe_linear_int4(float* y, const void* x, const uint8_t* x_scales, const uint
     if (rc) return rc;
     if (group != 32 && group != 64 && group != 128) return MOE_ERR_FORMAT;
     if ((uintptr_t)tiled_zeros & 15u) return MOE_ERR_ALIGN;
-    return launch_linear_w4({y, x, x_scales, tiled_codes, reinterpret_cast<const uint8_t*>(tiled_scales), tiled_zeros, bias, B, K, N}, group,
-                            as_stream(stream));
+    return launch_linear_w4({y, x, x_scales, tiled_codes, reinterpret_cast<const uint8_t*>(tiled_scales), tiled_zeros, bias, B, K, N, 0}, group,
+                            device_cu_count(), as_stream(stream));
 }
 
 // the repack's grids count 256 lanes, and scales, to a block

@@ -145,6 +145,12 @@ MOE_DEVICE double wave_sum(double v) {
     return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
+// LDS written by some lanes of a wave is read by others after this: the hardware keeps a wave's LDS accesses in order, the compiler has to.
+MOE_DEVICE void lds_in_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // ---- clamped SwiGLU (src/run.cpp:673-689) ---------------------------------------------------
 MOE_DEVICE float swiglu(float gate, float up, float alpha, float limit) {
     gate = gate > limit ? limit : gate;

@@ -200,8 +200,9 @@ struct LinearArgs {
     const uint8_t* w_zeros;   // int4: or nullptr (8 everywhere)
     const uint16_t* bias;     // bf16 [N], or nullptr
     int B, K, N;
+    int wide_stores;          // four values of y at a time (set by the launcher)
 };
-int launch_linear_w4(const LinearArgs& a, int group, hipStream_t stream);  // group: 0 MXFP4, else of the int4 scales
+int launch_linear_w4(const LinearArgs& a, int group, int n_cus, hipStream_t stream);  // group: 0 MXFP4, else of the int4 scales
 void int4_tiled_bytes(int rows, int K, int group, size_t* codes, size_t* scales, size_t* zeros);
 int launch_int4_repack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int rows, int K, int group, uint8_t* tiled_codes,
                        uint16_t* tiled_scales, uint8_t* tiled_zeros, hipStream_t stream);

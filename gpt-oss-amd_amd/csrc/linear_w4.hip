@@ -1,4 +1,5 @@
 // Products of a few rows with a matrix of 4-bit weights and group scales: y[b, n] = bias[n] + sum_k x[b, k] W[n, k].
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -8,7 +9,10 @@ namespace moe {
 
 namespace {
 
-constexpr int kLinearWaves = 8;
+constexpr int kUnit = 256;      // contraction elements of a wave: two chunks of 128
+
+// Waves of a block at most: what the registers of a wave allow (16: 128, 12: 168, 8: 256).
+constexpr int max_waves(int group, int nt) { return group == 32 && nt == 2 ? 8 : nt == 1 && (group == 0 || group == 128) ? 16 : 12; }
 
 // e4m3 values times a power of two, to bf16 (exact: three mantissa bits).
 MOE_DEVICE u32x4 e4m3x8_to_bf16(uint32_t lo, uint32_t hi, float scale) {
@@ -20,6 +24,86 @@ MOE_DEVICE u32x4 e4m3x8_to_bf16(uint32_t lo, uint32_t hi, float scale) {
     return v;
 }
 
+// Floats of the LDS that a wave keeps its partial tiles in, those of two steps; a chunk of 16 rows of x goes through it while it is loaded.
+__host__ __device__ constexpr int part_floats(int nt, int tiles_per_step) { return 2 * tiles_per_step * nt > 4 ? 2 * tiles_per_step * nt * 256 : 1024; }
+
+// Unit u of rows b0 .. b0 + 16 NT - 1 of x, as xr[chunk][MFMA step][token tile]: token q, 8 elements per lane, which are 32 g + 8 j .. of the chunk
+// for MXFP4 weights and 32 j + 8 g .. for int4.  Loaded in whole lines, 16 bytes of consecutive lanes side by side, and brought to the
+// lanes that need them through `bounce`, 4 KiB of LDS of this wave alone: loads whose lanes follow the operand layout run at a quarter of
+// the rate.  Rows past the last and elements past K are zeros (reads past a buffer's end).
+template <int GROUP, int NT>
+MOE_DEVICE void load_x(const LinearArgs& a, uint8_t* bounce, int b0, int u, u32x4 (&xr)[2][4][NT]) {
+    const int lane = threadIdx.x & 63;
+    const int q = lane & 15, g = lane >> 4;
+    const uint32_t rows = (uint32_t)min(a.B - b0, 16 * NT), K = (uint32_t)a.K;
+    constexpr uint32_t kOutside = 0x80000000u;  // rows * K * 2 < 2^31
+    if (a.x_scales == nullptr) {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t*>(static_cast<const uint16_t*>(a.x) + (size_t)b0 * K), 0, (int)(rows * K * 2), 0x00020000);
+        // four rows of 256 bytes to an instruction
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t k = kUnit * u + 128 * i + 8 * q;
+            const uint32_t at = k < K ? (g * K + k) * 2 : kOutside;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) xr[i][n][t] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)at, (int)((16 * t + 4 * n) * K * 2), 0);
+        }
+        // piece c (of 16) of row r at position c ^ r of the row's 256 bytes: no two lanes of a read meet in a bank
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int n = 0; n < 4; ++n) *reinterpret_cast<u32x4*>(bounce + (4 * n + g) * 256 + ((q ^ (4 * n + g)) << 4)) = xr[i][n][t];
+                lds_in_order();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) xr[i][j][t] = *reinterpret_cast<const u32x4*>(bounce + q * 256 + (((GROUP ? 4 * j + g : 4 * g + j) ^ q) << 4));
+                lds_in_order();
+            }
+    } else {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(static_cast<const uint8_t*>(a.x) + (size_t)b0 * K), 0, (int)(rows * K), 0x00020000);
+        const __amdgpu_buffer_rsrc_t s_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(a.x_scales + (size_t)b0 * (K / 32)), 0, (int)(rows * (K / 32)), 0x00020000);
+        // eight rows of 128 bytes to an instruction; the scale of the lane's row q and 32 elements g
+        u32x4 c[2][2][NT];
+        uint32_t s[2][NT];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t k = kUnit * u + 128 * i + 16 * (lane & 7), ks = kUnit * u + 128 * i + 32 * g;
+            const uint32_t at = k < K ? (uint32_t)(lane >> 3) * K + k : kOutside, at_s = ks < K ? q * (K / 32) + ks / 32 : kOutside;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) c[i][n][t] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)at, (int)((16 * t + 8 * n) * K), 0);
+                s[i][t] = __builtin_amdgcn_raw_buffer_load_b8(s_rsrc, (int)at_s, (int)(16 * t * (K / 32)), 0);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                // piece p (of 8) of row r at position p ^ (r / 2) of the row's 128 bytes
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int r = 8 * n + (lane >> 3);
+                    *reinterpret_cast<u32x4*>(bounce + r * 128 + (((lane & 7) ^ (r >> 1)) << 4)) = c[i][n][t];
+                }
+                lds_in_order();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = GROUP ? 32 * j + 8 * g : 32 * g + 8 * j;  // of 128, a byte each
+                    const uint2 v = *reinterpret_cast<const uint2*>(bounce + q * 128 + (((e >> 4) ^ (q >> 1)) << 4) + (e & 8));
+                    const uint32_t sb = GROUP ? (uint32_t)__shfl((int)s[i][t], 16 * j + q) : s[i][t];
+                    xr[i][j][t] = e4m3x8_to_bf16(v.x, v.y, mxfp4_scale_to_f32(sb));
+                }
+                lds_in_order();
+            }
+    }
+}
+
 // Eight codes 0..15 of a dword (order of int4_repack_kernel) as the bf16 numbers 16..31: the code goes to the mantissa's top four bits.
 MOE_DEVICE u32x4 int4_dword_to_bf16x8(uint32_t w) {
     constexpr uint32_t kMask = 0x00780078u, kSixteen = 0x41804180u;
@@ -28,129 +112,351 @@ MOE_DEVICE u32x4 int4_dword_to_bf16x8(uint32_t w) {
 
 }  // namespace
 
-// GROUP 0: MXFP4 weights in the tiled layout of mxfp4.hip; else int4 codes with a scale per GROUP values (layout of int4_repack_kernel).
-// A block takes a tile of 16 weight rows against 16 NT rows of x; its waves share the contraction, in chunks of 128, and meet in LDS.
-template <int GROUP, int NT, bool MX8>
-__global__ __launch_bounds__(64 * kLinearWaves) void linear_w4_kernel(LinearArgs a) {
-    __shared__ __attribute__((aligned(16))) float part[kLinearWaves][NT * 256];
+// The weights of one unit of a tile as they come from memory.
+template <int GROUP>
+struct UnitWeights {
+    static constexpr int kGroups = GROUP ? kUnit / GROUP : 1;
+    u32x4 raw[2];
+    uint32_t sw;                      // MXFP4: the scale bytes of four chunks
+    u32x4 sc[GROUP ? kGroups / 2 : 1];  // int4: four rows' scales of two groups
+    u32x2 zp[GROUP ? kGroups / 2 : 1];  // and their zero points
+
+    // Unit u of a tile; nothing is read unless `in`, without a branch: the compiler would wait for every load in flight where two paths meet.
+    MOE_DEVICE void load(const LinearArgs& a, int tile, int u, bool in) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        const int n_chunks = ceil_div(a.K, 128), n_units = ceil_div(a.K, kUnit);
+        const uint32_t tile_bytes = GROUP ? (uint32_t)n_chunks * 1024u : (uint32_t)(a.K / 32) * 256u;
+        const uint32_t scale_bytes = GROUP ? (uint32_t)n_units * (kGroups * 32u) : (uint32_t)ceil_div(n_chunks, 4) * 256u;
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.w) + (size_t)(uint32_t)tile * tile_bytes, 0,
+                                                                              in ? (int)tile_bytes : 0, 0x00020000);
+        const __amdgpu_buffer_rsrc_t s_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(a.w_scales) + (size_t)(uint32_t)tile * scale_bytes, 0, in ? (int)scale_bytes : 0, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) raw[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane * 16, (2 * u + i) * 1024, 2 /* nt */);
+        if constexpr (GROUP == 0) {
+            sw = __builtin_amdgcn_raw_buffer_load_b32(s_rsrc, lane * 4, (u >> 1) * 256, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kGroups / 2; ++i)
+                sc[i] = __builtin_amdgcn_raw_buffer_load_b128(s_rsrc, g * kGroups * 8 + i * 16, u * kGroups * 32, 0);
+            const __amdgpu_buffer_rsrc_t z_rsrc =
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.w_zeros) + (size_t)(uint32_t)tile * (scale_bytes / 2), 0,
+                                                  in && a.w_zeros ? (int)(scale_bytes / 2) : 0, 0x00020000);
+#pragma unroll
+            for (int i = 0; i < kGroups / 2; ++i)
+                zp[i] = __builtin_amdgcn_raw_buffer_load_b64(z_rsrc, g * kGroups * 4 + i * 8, u * kGroups * 16, 0);
+        }
+    }
+
+    // acc = the unit's products with x, from zero
+    template <int NT>
+    MOE_DEVICE void multiply(bool zeros, int u, const u32x4 (&xr)[2][4][NT], const float (&sum_x)[kGroups][NT], f32x4 (&acc)[NT]) const {
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t] = zero;
+        if constexpr (GROUP == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                // reads past the tile give 0, and the scale bytes of blocks that do not exist are 0
+                const float s = mxfp4_scale_to_f32((sw >> (16 * (u & 1) + 8 * i)) & 0xFFu);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t d[4];
+                    mxfp4_dword_to_bf16x8(raw[i][j], s, d);
+                    const u32x4 av = {d[0], d[1], d[2], d[3]};
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) acc[t] = mfma_16x16x32(av, xr[i][j][t], acc[t]);
+                }
+            }
+        } else {
+            // sum x (q - z) s = s (sum x (16 + q) - (16 + z) sum x) per group: 16 + q is a bf16 number
+            f32x4 p[NT];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const u32x4 av = int4_dword_to_bf16x8(raw[n >> 2][n & 3]);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) p[t] = mfma_16x16x32(av, xr[n >> 2][n & 3][t], 32 * n % GROUP == 0 ? zero : p[t]);
+                if (32 * (n + 1) % GROUP == 0) {
+                    const int grp = 32 * n / GROUP;
+                    const uint32_t zb = zeros ? zp[grp / 2][grp & 1] : 0x18181818u;
+                    const uint32_t s01 = sc[grp / 2][2 * (grp & 1)], s23 = sc[grp / 2][2 * (grp & 1) + 1];
+                    const float s[4] = {bf16_bits_to_f32(s01 & 0xFFFFu), bf16_bits_to_f32(s01 >> 16), bf16_bits_to_f32(s23 & 0xFFFFu),
+                                        bf16_bits_to_f32(s23 >> 16)};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float z = (float)((zb >> (8 * r)) & 0xFFu);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) acc[t][r] = fmaf(s[r], fmaf(-z, sum_x[grp][t], p[t][r]), acc[t][r]);
+                    }
+                    if (GROUP < 128) __builtin_amdgcn_sched_barrier(0);  // or all groups' factors are made first, and spilled
+                }
+            }
+        }
+    }
+};
+
+// Sums of x over the groups of a unit, by a product with ones: every row of the result is the sums of its columns.
+template <int GROUP, int NT>
+MOE_DEVICE void group_sums(const u32x4 (&xr)[2][4][NT], float (&sum_x)[UnitWeights<GROUP>::kGroups][NT]) {
+    if constexpr (GROUP != 0) {
+        const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            f32x4 s;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                if (32 * n % GROUP == 0) s = f32x4{0.f, 0.f, 0.f, 0.f};
+                s = mfma_16x16x32(ones, xr[n >> 2][n & 3][t], s);
+                if (32 * (n + 1) % GROUP == 0) sum_x[32 * n / GROUP][t] = s[0];
+            }
+        }
+    }
+}
+
+// Weight row of row r of a tile.
+template <int GROUP>
+MOE_DEVICE int weight_row(int tile, int r) {
+    return GROUP ? tile * 16 + r : (tile >> 2) * 64 + tile_row_in_group(tile & 3, r);
+}
+
+// Four results of token b from weight row n on.
+MOE_DEVICE void store_results(const LinearArgs& a, int b, int n, const f32x4& v) {
+    float* const dst = a.y + (size_t)b * a.N + n;
+    if (a.wide_stores) {  // N is a multiple of four
+        if (n < a.N) *reinterpret_cast<f32x4*>(dst) = v;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (n + r < a.N) dst[r] = v[r];
+    }
+}
+
+MOE_DEVICE f32x4 load_bias(const LinearArgs& a, int n) {  // 0 without one, and past N
+    const __amdgpu_buffer_rsrc_t rsrc =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.bias), 0, a.bias ? a.N * 2 : 0, 0x00020000);
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = bf16_bits_to_f32((uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rsrc, (n + r) * 2, 0, 0));
+    return v;
+}
+
+// Few tiles: a block for each, its waves take the units in turn.  Such a launch is a chain of latencies (arguments, weights and rows, LDS
+// and back, the waves' meeting, stores), so its code is short and nothing waits before the first loads are out.
+template <int GROUP, int NT>
+__global__ __launch_bounds__(64 * max_waves(GROUP, NT)) void linear_tile_kernel(LinearArgs a) {
+    extern __shared__ __attribute__((aligned(16))) float lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int q = lane & 15, g = lane >> 4;
-    const int tile = blockIdx.x, K = a.K;
-    const int n_chunks = ceil_div(K, 128);
-    const int per_wave = ceil_div(n_chunks, kLinearWaves);
-    const int c0 = wave * per_wave, c1 = min(c0 + per_wave, n_chunks);
-    const uint32_t tile_bytes = GROUP ? (uint32_t)n_chunks * 1024u : (uint32_t)(K / 32) * 256u;
-    const __amdgpu_buffer_rsrc_t w_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(a.w) + (size_t)tile * tile_bytes, 0, (int)tile_bytes, 0x00020000);
-    int tok[NT];
+    const int waves = blockDim.x >> 6;
+    const int tile = blockIdx.z * 8 + blockIdx.x, b0 = blockIdx.y * 16 * NT;
+    const int n_units = ceil_div(a.K, kUnit);
+    float* const part = lds;  // [n_units][NT][256]
+    uint8_t* const bounce = reinterpret_cast<uint8_t*>(lds + n_units * NT * 256) + wave * 4096;
+    if (tile * 16 >= a.N) return;
+    for (int u = wave; u < n_units; u += waves) {
+        UnitWeights<GROUP> w;
+        w.load(a, tile, u, true);
+        u32x4 xr[2][4][NT];
+        load_x<GROUP, NT>(a, bounce, b0, u, xr);
+        float sum_x[UnitWeights<GROUP>::kGroups][NT];
+        group_sums<GROUP, NT>(xr, sum_x);
+        f32x4 acc[NT];
+        w.template multiply<NT>(a.w_zeros != nullptr, u, xr, sum_x, acc);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) tok[t] = min((int)blockIdx.y * 16 * NT + t * 16 + q, a.B - 1);
-    // the 8 contraction elements of MFMA step j for this lane: their first
-    auto elem = [&](int c, int j) { return 128 * c + (GROUP ? 32 * j + 8 * g : 32 * g + 8 * j); };
-    auto x_frag = [&](int c, int j, int t) {
-        const int k = elem(c, j);
-        if (k >= K) return u32x4{0u, 0u, 0u, 0u};
-        if constexpr (MX8) {
-            const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.x) + (size_t)tok[t] * K + k);
-            const float s = mxfp4_scale_to_f32(a.x_scales[(size_t)tok[t] * (K / 32) + k / 32]);
-            return e4m3x8_to_bf16(v.x, v.y, s);
-        } else {
-            return *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.x) + (size_t)tok[t] * K + k);
-        }
-    };
-    f32x4 acc[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int c = c0; c < c1; ++c) {
-        const u32x4 raw = __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, lane * 16, c * 1024, 2 /* nt */);
-        if constexpr (GROUP == 0) {
-            // reads past the tile give 0, and the scale bytes of blocks that do not exist are 0
-            const uint32_t sw = *reinterpret_cast<const uint32_t*>(a.w_scales + (size_t)tile * ceil_div(n_chunks, 4) * 256 +
-                                                                   (c >> 2) * 256 + lane * 4);
-            const float sc = mxfp4_scale_to_f32((sw >> (8 * (c & 3))) & 0xFFu);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t d[4];
-                mxfp4_dword_to_bf16x8(raw[j], sc, d);
-                const u32x4 av = {d[0], d[1], d[2], d[3]};
-#pragma unroll
-                for (int t = 0; t < NT; ++t) acc[t] = mfma_16x16x32(av, x_frag(c, j, t), acc[t]);
-            }
-        } else {
-            // sum x (q - z) s = s (sum x (16 + q) - (16 + z) sum x) per group: 16 + q is a bf16 number, and the sum of x comes from a
-            // product with ones
-            const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
-            const int n_groups = ceil_div(K, GROUP);
-            f32x4 part_g[NT], sum_x[NT];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool first = 32 * j % GROUP == 0, last = 32 * (j + 1) % GROUP == 0;
-                const u32x4 av = int4_dword_to_bf16x8(raw[j]);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const u32x4 xv = x_frag(c, j, t);
-                    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-                    part_g[t] = mfma_16x16x32(av, xv, first ? zero : part_g[t]);
-                    sum_x[t] = mfma_16x16x32(ones, xv, first ? zero : sum_x[t]);
-                }
-                const int grp = (128 * c + 32 * j) / GROUP;
-                if (last && grp < n_groups) {
-                    const size_t at = ((size_t)tile * n_groups + grp) * 16 + 4 * g;
-                    const uint2 sb = *reinterpret_cast<const uint2*>(a.w_scales + 2 * at);
-                    const uint32_t zb = a.w_zeros ? *reinterpret_cast<const uint32_t*>(a.w_zeros + at) : 0x18181818u;
-                    const float s[4] = {bf16_bits_to_f32(sb.x & 0xFFFFu), bf16_bits_to_f32(sb.x >> 16), bf16_bits_to_f32(sb.y & 0xFFFFu),
-                                        bf16_bits_to_f32(sb.y >> 16)};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float z = (float)((zb >> (8 * i)) & 0xFFu);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) acc[t][i] = fmaf(s[i], fmaf(-z, sum_x[t][i], part_g[t][i]), acc[t][i]);
-                    }
-                }
-            }
-        }
+        for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(part + (u * NT + t) * 256 + lane * 4) = acc[t];
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(&part[wave][t * 256 + q * 16 + 4 * g]) = acc[t];
+    const int n = weight_row<GROUP>(tile, 4 * (lane >> 4));
+    f32x4 bias = {0.f, 0.f, 0.f, 0.f};
+    if (wave < NT) bias = load_bias(a, n);
     __syncthreads();
-    for (int i = threadIdx.x; i < NT * 256; i += 64 * kLinearWaves) {
-        float v = 0.f;
+    for (int t = wave; t < NT; t += waves) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int u = 0; u < n_units; ++u) v += *reinterpret_cast<const f32x4*>(part + (u * NT + t) * 256 + lane * 4);
+        const int b = b0 + t * 16 + (lane & 15);
+        if (b < a.B) store_results(a, b, n, v + bias);
+    }
+}
+
+// How a launch is cut: a block has wk x wr waves; the contraction's units are dealt out over wk waves, in as many slabs as that takes, and its
+// tiles of 16 weight rows, tiles_per_block consecutive ones, over wr.
+struct LinearCut {
+    int wk, log_wr, n_slabs, tiles_per_block;
+    int tiles_per_step;  // tile sets between two barriers that there is room for
+};
+
+// GROUP 0: MXFP4 weights in the tiled layout of mxfp4.hip; else int4 codes with a scale per GROUP values (layout of int4_repack_kernel).
+// A wave holds its unit of 16 NT rows of x in registers and goes through the block's tiles, the weights of the next D in flight; the waves of
+// a tile meet in LDS and one of them, another for every tile, adds up.  A result is the sum over units in ascending order, whatever the
+// cut: it does not depend on how many rows x has.
+template <int GROUP, int NT, int D, int G>
+__global__ __launch_bounds__(64 * max_waves(GROUP, NT)) void linear_w4_kernel(LinearArgs a, LinearCut cut) {
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    constexpr int kPart = NT * 256;                     // values of a tile
+    // grid (8, token blocks, tile blocks / 8): token blocks of the same weights side by side on one XCD; no quotient is formed in here, each is
+    // a chain of forty instructions, and a launch for one row is little more than a few chains
+    const int lane = threadIdx.x & 63;
+    const int wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = __builtin_amdgcn_readfirstlane(threadIdx.y);
+    const int n_wr = 1 << cut.log_wr, waves = cut.wk << cut.log_wr, wave = wr * cut.wk + wk;
+    const int q = lane & 15, g = lane >> 4;
+    const int n_units = ceil_div(a.K, kUnit);
+    const int n_tiles = ceil_div(a.N, 16);
+    const int token_block = blockIdx.y, tile_block = blockIdx.z * 8 + blockIdx.x;
+    const int tile0 = tile_block * cut.tiles_per_block, tile1 = min(tile0 + cut.tiles_per_block, n_tiles);
+    if (tile0 >= n_tiles) return;
+    const int n_slabs = cut.n_slabs;
+    // a wave's partial tiles, G of them in either half; x goes through the first while it is loaded
+    const int per_wave = part_floats(NT, cut.tiles_per_step);
+    float* const part = lds;                              // [waves][2][tiles_per_step][kPart]
+    float* const bias = lds + waves * per_wave;           // [tiles_per_block][16]
+    float* const sums = bias + cut.tiles_per_block * 16;    // [tiles_per_block][kPart] between slabs
+    const int b0 = token_block * 16 * NT;
+    const int n_bias = (tile1 - tile0) * 16;
+    for (int i = 64 * wave + lane; i < n_bias; i += 64 * waves) {
+        const int n = weight_row<GROUP>(tile0 + (i >> 4), i & 15);
+        bias[i] = a.bias && n < a.N ? bf16_bits_to_f32(a.bias[n]) : 0.f;
+    }
+    UnitWeights<GROUP> w[D];
+
+    int half = 0, turn = 0;  // which half of `part` a step writes, and which wave adds up its first item
+    for (int slab = 0; slab < n_slabs; ++slab) {
+        const int u = slab * cut.wk + wk;
+        auto load_slot = [&](int d, int tile) { w[d].load(a, min(tile, n_tiles - 1), u, tile < tile1 && u < n_units); };
+        load_slot(0, tile0 + wr);
+        u32x4 xr[2][4][NT];
+        load_x<GROUP, NT>(a, reinterpret_cast<uint8_t*>(part + wave * per_wave), b0, u, xr);
+        __builtin_amdgcn_sched_barrier(0);  // the other slots' registers are free until x is where it stays
 #pragma unroll
-        for (int w = 0; w < kLinearWaves; ++w) v += part[w][i];
-        const int r = i & 15;  // row of the tile
-        const int n = GROUP ? tile * 16 + r : (tile >> 2) * 64 + tile_row_in_group(tile & 3, r);
-        const int b = (int)blockIdx.y * 16 * NT + (i >> 4);
-        if (b < a.B && n < a.N) {
-            if (a.bias) v += bf16_bits_to_f32(a.bias[n]);
-            a.y[(size_t)b * a.N + n] = v;
+        for (int d = 1; d < D; ++d) load_slot(d, tile0 + wr + d * n_wr);
+        float sum_x[UnitWeights<GROUP>::kGroups][NT];
+        group_sums<GROUP, NT>(xr, sum_x);
+        // partial tile of slot S of the ring, the M-th of its step
+        auto tile_part = [&](auto slot_tag, int m, int tile) {
+            constexpr int S = decltype(slot_tag)::value;
+            f32x4 acc[NT];
+            w[S].template multiply<NT>(a.w_zeros != nullptr, u, xr, sum_x, acc);
+            __builtin_amdgcn_sched_barrier(0);
+            load_slot(S, tile + D * n_wr);  // the slot is free
+            __builtin_amdgcn_sched_barrier(0);
+            if (tile - wr >= tile1) return;  // a set that is not this block's: block-uniform
+            float* const mine = part + wave * per_wave + ((half * cut.tiles_per_step) + m) * kPart;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(mine + t * 256 + lane * 4) = acc[t];
+        };
+        // The G tile sets from `tile` on: item (m, w, t), token tile t of the m-th tile of row wave w, is added up by one wave; the items of
+        // the steps go round over the waves.
+        auto add_up = [&](int tile) {
+            __syncthreads();
+            const int units = min(cut.wk, n_units - slab * cut.wk);
+            const int items = max(0, min(G << cut.log_wr, tile1 - tile)) * NT;
+            auto add = [&](int item) {
+                const int set = item / NT, t = item - set * NT;
+                const int m = set >> cut.log_wr, w = set & (n_wr - 1);
+                const int tl = tile + set;  // wave-uniform
+                const float* src = part + w * cut.wk * per_wave + (half * cut.tiles_per_step + m) * kPart + t * 256 + lane * 4;
+                float* const between = sums + (tl - tile0) * kPart + t * 256 + lane * 4;
+                f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                if (slab > 0) v = *reinterpret_cast<const f32x4*>(between);
+#pragma unroll 4
+                for (int i = 0; i < units; ++i) v += *reinterpret_cast<const f32x4*>(src + i * per_wave);
+                if (slab + 1 < n_slabs) {
+                    *reinterpret_cast<f32x4*>(between) = v;
+                    return;
+                }
+                const int b = b0 + t * 16 + q;
+                if (b >= a.B) return;
+                v += *reinterpret_cast<const f32x4*>(bias + (tl - tile0) * 16 + 4 * g);
+                store_results(a, b, weight_row<GROUP>(tl, 4 * g), v);
+            };
+            // without a loop where one round does: in front of a loop that stores, the compiler waits for every load in flight
+            int item = wave - turn;
+            if (item < 0) item += waves;
+            if (item < items) add(item);
+            if (items > waves)
+                for (item += waves; item < items; item += waves) add(item);
+            turn += items;
+            while (turn >= waves) turn -= waves;
+            half ^= 1;
+        };
+        // the ring's slots are constants: D or G tile sets, whichever is more, to a pass of the loop
+        for (int tile = tile0; tile < tile1; tile += (D > G ? D : G) * n_wr) {
+            auto at = [&](auto m_tag) {
+                constexpr int M = decltype(m_tag)::value;
+                if constexpr (M < (D > G ? D : G)) {
+                    tile_part(std::integral_constant<int, M % D>{}, M % G, tile + M * n_wr + wr);
+                    if constexpr (M % G == G - 1) add_up(tile + (M - G + 1) * n_wr);
+                }
+            };
+            at(std::integral_constant<int, 0>{});
+            at(std::integral_constant<int, 1>{});
+            at(std::integral_constant<int, 2>{});
+            at(std::integral_constant<int, 3>{});
         }
+        if (slab + 1 < n_slabs) __syncthreads();  // the next slab's x goes through `part`
     }
 }
 
-template <int GROUP>
-static int launch_linear_of(const LinearArgs& a, hipStream_t stream) {
-    const unsigned tiles = (unsigned)ceil_div(a.N, 16);
-    auto launch = [&](auto kernel, int nt) {
-        hipLaunchKernelGGL(kernel, dim3(tiles, ceil_div(a.B, 16 * nt)), dim3(64 * kLinearWaves), 0, stream, a);
-        return launch_status();
+constexpr size_t kLdsMost = 160 * 1024;
+
+// A block for each tile: n_units partial tiles and 4 KiB a wave in LDS.
+static size_t linear_tile_lds(int group, int nt, int n_units) {
+    return (size_t)n_units * nt * 1024 + (size_t)std::min(n_units, max_waves(group, nt)) * 4096;
+}
+
+template <int GROUP, int NT>
+static int launch_linear_tile(const LinearArgs& a, int n_units, hipStream_t stream) {
+    const int waves = std::min(n_units, max_waves(GROUP, NT));
+    hipLaunchKernelGGL((linear_tile_kernel<GROUP, NT>), dim3(8, ceil_div(a.B, 16 * NT), ceil_div(ceil_div(a.N, 16), 8)), dim3(64 * waves),
+                       linear_tile_lds(GROUP, NT, n_units), stream, a);
+    return launch_status();
+}
+
+template <int GROUP, int NT, int D, int G>
+static int launch_linear_of(const LinearArgs& a, int n_cus, hipStream_t stream) {
+    const int n_tiles = ceil_div(a.N, 16), n_units = ceil_div(a.K, kUnit);
+    LinearCut cut;
+    const int slabs = ceil_div(n_units, max_waves(GROUP, NT));
+    cut.n_slabs = slabs;
+    cut.wk = ceil_div(n_units, slabs);
+    cut.log_wr = 0;
+    while (cut.wk << (cut.log_wr + 1) <= 8 && n_tiles >> cut.log_wr > n_cus) ++cut.log_wr;
+    const int wr = 1 << cut.log_wr, waves = cut.wk * wr, token_blocks = ceil_div(a.B, 16 * NT);
+    const int at_once = n_cus * std::max(1, max_waves(GROUP, NT) / waves);
+    const int most = (slabs > 1 ? 32 / NT : 128) / wr;  // what the LDS has room for
+    cut.tiles_per_block = std::min(most, ceil_div(n_tiles * token_blocks, at_once * wr)) * wr;
+    cut.tiles_per_step = std::min(G, cut.tiles_per_block / wr);
+    const size_t lds = (size_t)waves * part_floats(NT, cut.tiles_per_step) * 4 + (size_t)cut.tiles_per_block * (64 + (slabs > 1 ? NT * 1024 : 0));
+    const int blocks = ceil_div(n_tiles, cut.tiles_per_block);
+    hipLaunchKernelGGL((linear_w4_kernel<GROUP, NT, D, G>), dim3(8, token_blocks, ceil_div(blocks, 8)), dim3(64 * cut.wk, wr), lds, stream, a, cut);
+    return launch_status();
+}
+
+// Which kernel: by the matrix and the number of rows alone, and all of them add in the same order.
+template <int GROUP, int NT>
+static int launch_linear_rows(const LinearArgs& a, int n_cus, hipStream_t stream) {
+    const int n_units = ceil_div(a.K, kUnit);
+    const long long tiles = (long long)ceil_div(a.N, 16) * ceil_div(a.B, 16 * NT);
+    if (tiles <= n_cus && linear_tile_lds(GROUP, NT, n_units) <= kLdsMost) return launch_linear_tile<GROUP, NT>(a, n_units, stream);
+    // with three tiles to a block the ring and the shared steps of the second form cost more code than they hide: us, first : second form, 1 row of
+    // 5760 x 2880 MXFP4 5.8 : 6.5, 16 rows of 16384 x 4096 11.9 : 11.2, of 131072 x 2880 45.7 : 38.9; more than 128 int4 scales a block of weights
+    // do not fit its registers: scales per 64, 32 rows, and per 32
+    if (tiles <= 3LL * n_cus || GROUP == 32 || (GROUP == 64 && NT == 2)) return launch_linear_of<GROUP, NT, 1, 2>(a, n_cus, stream);
+    if constexpr (!(GROUP == 32 || (GROUP == 64 && NT == 2))) return launch_linear_of<GROUP, NT, 2, 4 / NT>(a, n_cus, stream);
+    return MOE_ERR_LIMIT;
+}
+
+int launch_linear_w4(const LinearArgs& args, int group, int n_cus, hipStream_t stream) {
+    LinearArgs a = args;
+    a.wide_stores = a.N % 4 == 0 && ((uintptr_t)a.y & 15u) == 0;
+    auto rows = [&](auto g) {
+        constexpr int GROUP = decltype(g)::value;
+        return a.B <= 16 ? launch_linear_rows<GROUP, 1>(a, n_cus, stream) : launch_linear_rows<GROUP, 2>(a, n_cus, stream);
     };
-    if (a.x_scales) {
-        if (a.B <= 16) return launch(linear_w4_kernel<GROUP, 1, true>, 1);
-        if (a.B <= 32) return launch(linear_w4_kernel<GROUP, 2, true>, 2);
-        return launch(linear_w4_kernel<GROUP, 4, true>, 4);
-    }
-    if (a.B <= 16) return launch(linear_w4_kernel<GROUP, 1, false>, 1);
-    if (a.B <= 32) return launch(linear_w4_kernel<GROUP, 2, false>, 2);
-    return launch(linear_w4_kernel<GROUP, 4, false>, 4);
-}
-
-int launch_linear_w4(const LinearArgs& a, int group, hipStream_t stream) {
     switch (group) {
-        case 0: return launch_linear_of<0>(a, stream);
-        case 32: return launch_linear_of<32>(a, stream);
-        case 64: return launch_linear_of<64>(a, stream);
-        case 128: return launch_linear_of<128>(a, stream);
+        case 0: return rows(std::integral_constant<int, 0>{});
+        case 32: return rows(std::integral_constant<int, 32>{});
+        case 64: return rows(std::integral_constant<int, 64>{});
+        case 128: return rows(std::integral_constant<int, 128>{});
     }
     return MOE_ERR_FORMAT;
 }
@@ -158,10 +464,10 @@ int launch_linear_w4(const LinearArgs& a, int group, hipStream_t stream) {
 // ---- int4 codes ------------------------------------------------------------------------------------
 // Tiles of 16 weight rows, a tile's contraction in chunks of 128 elements (the last one filled up with zeros), lane 16 g + r of a chunk's
 // 1 KiB: dword j holds elements 32 j + 8 g .. + 8 of row r, the element pair 2p, 2p + 1 at bits 4p and 16 + 4p, so that a shift and a mask leave a
-// pair at the same place of a dword's two halves.  Scales [tile][group][16] bf16, zero points [tile][group][16] as the byte 16 + z; 0 past the
-// last row.
+// pair at the same place of a dword's two halves.  Scales bf16, zero points as the byte 16 + z, both [tile][unit of 256][4 lane groups]
+// [groups of the unit][4 rows]: a lane reads those of the four rows it gets from the matrix instruction in one piece; 0 past the last row and group.
 void int4_tiled_bytes(int rows, int K, int group, size_t* codes, size_t* scales, size_t* zeros) {
-    const size_t tiles = (size_t)ceil_div(rows, 16), groups = (size_t)ceil_div(K, group);
+    const size_t tiles = (size_t)ceil_div(rows, 16), groups = (size_t)ceil_div(K, kUnit) * (kUnit / group);
     if (codes) *codes = tiles * (size_t)ceil_div(K, 128) * 1024;
     if (scales) *scales = tiles * groups * 32;
     if (zeros) *zeros = tiles * groups * 16;
@@ -190,13 +496,19 @@ __global__ __launch_bounds__(256) void int4_repack_kernel(const uint32_t* __rest
 
 __global__ __launch_bounds__(256) void int4_scales_repack_kernel(const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros,
                                                                  uint16_t* __restrict__ out_scales, uint8_t* __restrict__ out_zeros, int rows,
-                                                                 int n_groups, long long n) {
+                                                                 int K, int group, long long n) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
-    const long long tg = i >> 4, row = tg / n_groups * 16 + (i & 15);
-    const size_t src = (size_t)row * n_groups + (size_t)(tg % n_groups);
-    out_scales[i] = row < rows ? scales[src] : 0;
-    if (zeros) out_zeros[i] = row < rows ? (uint8_t)(16 + (zeros[src] & 15)) : 0;
+    const int per_unit = kUnit / group, n_units = ceil_div(K, kUnit), n_groups = ceil_div(K, group);
+    const long long unit = i / (16 * per_unit);  // over all tiles
+    const int in_unit = (int)(i - unit * (16 * per_unit));
+    const int g = in_unit / (4 * per_unit), grp = in_unit / 4 % per_unit;
+    const long long row = unit / n_units * 16 + 4 * g + (in_unit & 3);
+    const long long at = unit % n_units * per_unit + grp;
+    const bool in = row < rows && at < n_groups;
+    const size_t src = in ? (size_t)row * n_groups + (size_t)at : 0;
+    out_scales[i] = in ? scales[src] : 0;
+    if (zeros) out_zeros[i] = in ? (uint8_t)(16 + (zeros[src] & 15)) : 0;
 }
 
 int launch_int4_repack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int rows, int K, int group, uint8_t* tiled_codes,
@@ -204,10 +516,9 @@ int launch_int4_repack(const uint8_t* codes, const uint16_t* scales, const uint8
     const long long lanes = (long long)ceil_div(rows, 16) * ceil_div(K, 128) * 64;
     hipLaunchKernelGGL(int4_repack_kernel, dim3((unsigned)ceil_div(lanes, 256ll)), dim3(256), 0, stream,
                        reinterpret_cast<const uint32_t*>(codes), reinterpret_cast<u32x4*>(tiled_codes), rows, K, lanes);
-    const int groups = ceil_div(K, group);
-    const long long n = (long long)ceil_div(rows, 16) * groups * 16;
+    const long long n = (long long)ceil_div(rows, 16) * ceil_div(K, kUnit) * (kUnit / group) * 16;
     hipLaunchKernelGGL(int4_scales_repack_kernel, dim3((unsigned)ceil_div(n, 256ll)), dim3(256), 0, stream, scales, zeros, tiled_scales,
-                       tiled_zeros, rows, groups, n);
+                       tiled_zeros, rows, K, group, n);
     return launch_status();
 }
 

@@ -68,7 +68,7 @@ __global__ __launch_bounds__(256) void route_kernel(const float* __restrict__ lo
             keys[e] = key[c];
         }
     }
-    __builtin_amdgcn_wave_barrier();
+    lds_in_order();
     if (rule.n_groups > 1) {
         const int size = E / rule.n_groups;
         uint32_t first = 0, second = 0;

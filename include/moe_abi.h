@@ -299,7 +299,7 @@ MOE_API int moe_add_rmsnorm(float* x_out, const float* x, const float* delta, co
 
 /* y[b, n] = bias[n] + sum_k x[b, k] W[n, k], fp32 sums, for B rows and an N x K matrix; made for decode-sized batches (the weights are read
  * once per 64 rows).  x [B, K] is bf16 (x_scales NULL) or e4m3 codes with x_scales [B, K / 32] e8m0 as moe_add_rmsnorm writes them (byte 0
- * counts as a factor of 0, as in weights).  bias [N] bf16 or NULL.  K % 32 == 0, B <= 65535; x and the tiled tensors 16-byte aligned.
+ * counts as a factor of 0, as in weights).  bias [N] bf16 or NULL.  K % 32 == 0, K <= 2^24, B <= 65535; x and the tiled tensors 16-byte aligned.
  * Deterministic, and a row's result does not depend on the rows around it.
  *
  * moe_linear_mxfp4: tiled_blocks / tiled_scales of moe_mxfp4_repack(E = 1, rows = N, K); N % 64 == 0.

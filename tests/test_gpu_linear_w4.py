@@ -77,6 +77,19 @@ def test_exact_sums(pkg, dev, fmt, group, zeros, N, K):
 
 
 @pytest.mark.parametrize("fmt,group,zeros", FORMS)
+@pytest.mark.parametrize("N,K", [(4160, 96), (13056, 64), (20032, 288), (16448, 1184), (4800, 8224)])
+def test_exact_sums_of_many_tiles(pkg, dev, fmt, group, zeros, N, K):
+    """As above, for blocks that go through several tiles of weight rows: with waves side by side, the last block's tiles ending early, in one or
+    more slabs of the contraction; against sums in 64 bits on the device."""
+    w = Weights(pkg, dev, N, K, fmt, group, zeros, seed=N + K, exact=True)
+    wt = torch.from_numpy(w.w).to(dev).t().contiguous()
+    for B in (3, 20, 40):
+        print("exact sums", fmt, group, zeros, N, K, B, flush=True)
+        x = torch.randint(-4, 5, (B, K), device=dev, generator=torch.Generator(device=dev).manual_seed(B)).bfloat16()
+        assert torch.equal(w.run(x).double(), x.double() @ wt)
+
+
+@pytest.mark.parametrize("fmt,group,zeros", FORMS)
 @pytest.mark.parametrize("B,N,K", [(1, 2880, 2880), (5, 64, 4096), (16, 1024, 1440), (40, 640, 2880), (64, 2880, 640), (100, 128, 5760)])
 def test_against_64_bits(pkg, dev, fmt, group, zeros, B, N, K):
     w = Weights(pkg, dev, N, K, fmt, group, zeros, seed=B + N + K)

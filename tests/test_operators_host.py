@@ -75,8 +75,8 @@ def test_linear_refuses(pkg):
 
 
 def test_int4_repack_refuses_and_sizes(pkg):
-    assert pkg.int4_tiled_bytes(17, 160, 64) == (2 * 2 * 1024, 2 * 3 * 32, 2 * 3 * 16)
-    assert pkg.int4_tiled_bytes(16, 128, 128) == (1024, 32, 16)
+    assert pkg.int4_tiled_bytes(17, 160, 64) == (2 * 2 * 1024, 2 * 4 * 32, 2 * 4 * 16)
+    assert pkg.int4_tiled_bytes(16, 128, 128) == (1024, 2 * 32, 2 * 16)
     assert pkg.int4_tiled_bytes(0, 128, 128) == pkg.int4_tiled_bytes(16, 48, 32) == pkg.int4_tiled_bytes(16, 64, 48) == (0, 0, 0)
     f = pkg.lib.moe_int4_repack
     assert f(None, 16, None, 16, 64, 32, 16, 16, None, None) == f(16, 16, 16, 16, 64, 32, 16, 16, None, None) == -1
