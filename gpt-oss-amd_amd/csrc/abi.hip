@@ -205,6 +205,20 @@ const char* moe_error_string(int code) {
     }
 }
 
+// Compute units of the current device, asked once per device (the kernel choices below count rounds
+// of blocks over them).
+static int device_cu_count() {
+    static std::atomic<int> cached[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    int n = cached[dev].load(std::memory_order_relaxed);
+    if (n <= 0) {
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+        cached[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
 // ---- router ----------------------------------------------------------------------------------
 size_t moe_router_scratch_bytes(int N, int M) {
     if (N <= 0 || M <= 0) return 0;
@@ -285,7 +299,7 @@ int moe_route(float* topk_values, int* topk_indices, const float* router_logits,
     const int rc = check_route(rule, num_experts, experts_per_token);
     if (rc) return rc;
     return launch_route(router_logits, topk_values, topk_indices, batch_size, num_experts, experts_per_token, route_rule(rule),
-                        as_stream(stream));
+                        device_cu_count(), as_stream(stream));
 }
 
 // ---- bucketing -------------------------------------------------------------------------------
@@ -351,20 +365,6 @@ int moe_build_work_queue(const int* expert_offsets, int E, int* work_queue, int*
     if (!expert_offsets || !work_queue || !work_count) return MOE_ERR_NULL;
     if (E <= 0) return MOE_ERR_SHAPE;
     return launch_build_work_queue(expert_offsets, E, work_queue, work_count, as_stream(stream));
-}
-
-// Compute units of the current device, asked once per device (the kernel choices below count rounds
-// of blocks over them).
-static int device_cu_count() {
-    static std::atomic<int> cached[64];
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-    int n = cached[dev].load(std::memory_order_relaxed);
-    if (n <= 0) {
-        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-        cached[dev].store(n, std::memory_order_relaxed);
-    }
-    return n;
 }
 
 // Decode-sized buckets (producer/consumer kernel, one block per CU): 10 or 12 consumer waves of
@@ -906,7 +906,7 @@ static int block_forward_impl(const moe_block_params* caller, moe_stream_t strea
             }
             if (rc) return rc;
             if ((rc = mark())) return rc;
-            rc = launch_route(logits, p->topk_v, p->topk_i, T, E, K, route_rule(p->route), stream);
+            rc = launch_route(logits, p->topk_v, p->topk_i, T, E, K, route_rule(p->route), device_cu_count(), stream);
             break;
         }
     }

@@ -47,7 +47,8 @@ struct RouteRule {  // moe_route_params
     int scoring, n_groups, groups_per_token, group_top, renormalize;
     float scale;
 };
-int launch_route(const float* logits, float* topk_v, int* topk_i, int T, int E, int K, const RouteRule& rule, hipStream_t stream);
+int launch_route(const float* logits, float* topk_v, int* topk_i, int T, int E, int K, const RouteRule& rule, int n_cus,
+                 hipStream_t stream);
 
 // ---- bucket.hip -------------------------------------------------------------------------------
 // Token-block map consumed by the expert kernels: tile i covers rows

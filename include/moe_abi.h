@@ -129,7 +129,7 @@ MOE_API int moe_softmax(float* x, int batch_size, int size, moe_stream_t stream)
  *   groups    : experts form n_groups runs of num_experts / n_groups; a group's value is the sum (fp32) of its group_top largest choices
  *               (group_top 1 or 2; a group of one expert has one); the groups_per_token groups of largest value stay, equal ones: the lower
  *   chosen    : the experts_per_token largest choices of the groups that stay, in descending order, equal ones: the lower index.  A NaN
- *               counts as larger than any number.  The indices of a token are distinct and in range whatever its logits hold
+ *               counts as +infinity, a group's value too.  The indices of a token are distinct and in range whatever its logits hold
  *   value     = score[chosen], divided by the sum over the chosen if renormalize (0 where that sum is 0), times scale (fp64, rounded once)
  * num_experts <= 1024, a multiple of n_groups; n_groups <= 64; experts_per_token <= 8 and <= the experts of the groups that stay.  The
  * rule is host memory, read during the call; balance_bias [num_experts] is device memory or NULL. */

@@ -18,8 +18,8 @@ def scores(row, scoring):
 
 
 def ranked(values, allowed):
-    """Allowed indices by value, descending; equal ones ascending, NaN first."""
-    return sorted(allowed, key=lambda i: ((-np.inf if np.isnan(values[i]) else -values[i]), not np.isnan(values[i]), i))
+    """Allowed indices by value, descending; equal ones ascending, a NaN as +infinity."""
+    return sorted(allowed, key=lambda i: (-np.inf if np.isnan(values[i]) else -values[i], i))
 
 
 def route(logits, K, scoring="softmax", bias=None, n_groups=1, groups_per_token=1, group_top=1, renormalize=True, scale=1.0):

@@ -45,12 +45,28 @@ def test_route(pkg, dev, scoring, T, E, K):
 
 
 @pytest.mark.parametrize("E,G,keep,K", [(8, 8, 3, 3), (16, 2, 1, 8), (32, 4, 2, 4), (64, 8, 4, 6), (64, 64, 8, 8), (120, 5, 3, 8), (160, 8, 3, 6), (256, 8, 4, 8),
-                                        (256, 2, 2, 8), (512, 16, 1, 8), (960, 3, 2, 8), (1024, 64, 2, 8), (66, 33, 7, 8), (1000, 10, 10, 8)])
+                                        (256, 2, 2, 8), (512, 16, 1, 8), (960, 3, 2, 8), (1024, 64, 2, 8), (66, 33, 7, 8), (1000, 10, 10, 8), (990, 33, 4, 8),
+                                        (36, 3, 2, 5), (100, 10, 3, 8), (200, 2, 1, 7), (768, 2, 1, 8), (72, 9, 4, 6)])
 def test_route_groups(pkg, dev, E, G, keep, K):
     logits, bias = logits_of(37, E, E + G)
     for top in (1, 2):
         check(pkg, dev, logits, K, scoring="sigmoid", bias=bias, n_groups=G, groups_per_token=keep, group_top=top, scale=2.5)
     check(pkg, dev, logits, K, scoring="softmax", n_groups=G, groups_per_token=keep, renormalize=False)
+
+
+@pytest.mark.parametrize("T", [1601, 3307])  # 32 and 16 lanes to a token
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,G,keep,K", [(5, 1, 1, 2), (16, 4, 2, 4), (32, 1, 1, 4), (60, 5, 2, 6), (128, 8, 3, 8), (192, 8, 4, 8), (256, 8, 4, 8), (256, 1, 1, 8),
+                                        (258, 3, 2, 8), (400, 16, 5, 8), (512, 32, 3, 8), (768, 1, 1, 8), (1024, 8, 4, 8), (990, 33, 4, 8)])
+def test_many_tokens_as_few(pkg, dev, scoring, E, G, keep, K, T):
+    """Batches large enough for several tokens to a wave: the bits of the same rows in small batches, and those of the restatement."""
+    logits, bias = logits_of(T, E, E + G)
+    kw = dict(scoring=scoring, bias=bias, n_groups=G, groups_per_token=keep, group_top=2, scale=2.5)
+    v, i = run(pkg, dev, logits, K, **dict(kw))
+    for a, b in ((0, 30), (1000, 1031), (T - 33, T)):
+        sv, si = run(pkg, dev, logits[a:b].copy(), K, **dict(kw))
+        assert np.array_equal(i[a:b], si) and np.array_equal(v[a:b], sv)
+        check(pkg, dev, logits[a:b].copy(), K, **dict(kw))
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
@@ -66,8 +82,9 @@ def test_route_ties_go_to_the_lower_index(pkg, dev, scoring):
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
-@pytest.mark.parametrize("E,G,keep", [(16, 1, 1), (64, 8, 2), (256, 8, 4), (320, 4, 3)])
-def test_route_masked_and_far_logits(pkg, dev, scoring, E, G, keep):
+@pytest.mark.parametrize("T", [9, 1700, 3300])
+@pytest.mark.parametrize("E,G,keep", [(16, 1, 1), (64, 8, 2), (256, 8, 4), (320, 4, 3), (960, 3, 2)])
+def test_route_masked_and_far_logits(pkg, dev, scoring, E, G, keep, T):
     lowest = np.finfo(np.float32).min
     logits, bias = logits_of(9, E, E)
     logits[0] = -np.inf                  # nothing to choose from
@@ -84,7 +101,9 @@ def test_route_masked_and_far_logits(pkg, dev, scoring, E, G, keep):
         for renorm in (True, False):
             kw = dict(scoring=scoring, n_groups=G, groups_per_token=keep, group_top=2, renormalize=renorm)
             check(pkg, dev, logits, 4, bias=b, **kw)
-            v, i = run(pkg, dev, logits, 4, bias=b, **kw)
+            many = np.concatenate([logits, logits_of(T - 9, E, 1)[0]])
+            v, i = run(pkg, dev, many, 4, bias=b, **kw)
+            assert np.array_equal(i[:9], opsref.route(logits, 4, bias=b, **kw)[1])
             assert (i >= 0).all() and (i < E).all() and all(len(set(r)) == 4 for r in i)
     v, _ = run(pkg, dev, logits, 4, scoring="softmax")
     assert (v[0] == 0).all()
