@@ -49,27 +49,7 @@ MOE_DEVICE float4 fma4(const float4& v, float w, const float4& acc) {
 // NT: the rows by slot are more than the last-level cache holds and not in it any more; they are read past it.  e_agg is written past it
 // too: what the cache takes of it is written back during the launch after this one (the next call's router, 16384 tokens 125 us : 132 with the
 // loads alone : 121 with both; whole block 2624 : 2604 : 2594, 8192 tokens 1335 : 1324 : 1323; with the norm, stage and router together, 12000
-// tokens 324 : 298 : 278).
-template <bool NT>
-MOE_DEVICE float4 load_value(const float4* p) {
-    if constexpr (NT) {
-        const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-        return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
-    } else {
-        return *p;
-    }
-}
-
-template <bool NT>
-MOE_DEVICE void store_value(float4* p, const float4& v) {
-    if constexpr (NT) {
-        const u32x4 bits = {__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w)};
-        __builtin_nontemporal_store(bits, reinterpret_cast<u32x4*>(p));
-    } else {
-        *p = v;
-    }
-}
-
+// tokens 324 : 298 : 278).  load_value and store_value of common.h.
 // NI float4 columns (from c0, `step` apart, those below H4) of the token's combined row: K fused multiply-adds in ascending expert id.
 // slot_of == NULL: rows are stored by assignment, the row of (t, k) is t * K + k, known without looking at the routing, so
 // their loads go out together with the loads of the routing itself (one memory round trip instead of two).  The order of the

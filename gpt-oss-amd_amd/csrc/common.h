@@ -145,6 +145,27 @@ MOE_DEVICE double wave_sum(double v) {
     return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
+// ---- 16 bytes, past the caches if NT --------------------------------------------------------------
+template <bool NT>
+MOE_DEVICE float4 load_value(const float4* p) {
+    if constexpr (NT) {
+        const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+        return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+    } else {
+        return *p;
+    }
+}
+
+template <bool NT>
+MOE_DEVICE void store_value(float4* p, const float4& v) {
+    if constexpr (NT) {
+        const u32x4 bits = {__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w)};
+        __builtin_nontemporal_store(bits, reinterpret_cast<u32x4*>(p));
+    } else {
+        *p = v;
+    }
+}
+
 // LDS written by some lanes of a wave is read by others after this: the hardware keeps a wave's LDS accesses in order, the compiler has to.
 MOE_DEVICE void lds_in_order() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

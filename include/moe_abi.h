@@ -279,15 +279,14 @@ MOE_API int moe_rmsnorm(float* o, const float* x, const moe_bf16_t* weight, int 
 /* Residual add, RMSNorm and its result in the type that the next product reads (no counterpart in the reference, whose products read
  * fp32 rows):
  *   x_out = x + delta (fp32; x without a delta),  y = RMSNorm(x_out) with the arithmetic of moe_rmsnorm and the caller's eps
- * and of y what is asked for, at least one: o [batch, size] fp32; o_bf16 [batch, size] (round to nearest even); q [batch, size] e4m3 codes
- * with q_scales, value = code * scale:
- *   q_group 32   e8m0 bytes [batch, size / 32]: the smallest power of two, from 2^-126, that leaves the largest |y| of the 32 at 448 or
+ * and of y what is asked for, at least one: o [batch, size] fp32; o_bf16 [batch, size] (o rounded to nearest even); q [batch, size] e4m3
+ * codes with q_scales, value = code * scale, the code being the nearest (ties to even) to the quotient of y, before its rounding to fp32, and:
+ *   q_group 32   e8m0 bytes [batch, size / 32]: the smallest power of two, from 2^-126, that leaves the largest |o| of the 32 at 448 or
  *                below (byte b stands for 2^(b - 127)); size % 32 == 0.  What moe_linear_mxfp4 and moe_linear_int4 take as x, x_scales
- *   q_group 128  fp32 [batch, ceil(size / 128)], the last group may be shorter;  q_group 0  fp32 [batch], one a row:
- *                a = max(largest |y|, 2^-100), scale = a / 448, code = e4m3(y * (448 / a))
- * Codes are rounded to nearest even.  A group that holds an infinity or a NaN has a NaN for its scale and for every code.  x_out may be x;
- * otherwise no output may overlap an input.  size % 4 == 0; x, x_out, delta and o 16-byte aligned, weight and o_bf16 8-byte, q and fp32 scales
- * 4-byte. */
+ *   q_group 128  the largest |y| of the group, 2^-100 at least, over 448; the last group may be shorter.  Scales fp32
+ *                [batch, ceil(size / 128)]: that |y| in fp32, divided in fp32.  q_group 0 the same with one group a row, scales [batch]
+ * A group that holds an infinity or a NaN has a NaN for its scale and for every code.  x_out may be x; otherwise no output may overlap an
+ * input.  size % 4 == 0; x, x_out, delta and o 16-byte aligned, weight and o_bf16 8-byte, q and fp32 scales 4-byte. */
 enum { MOE_Q_GROUP_ROW = 0, MOE_Q_GROUP_MX = 32, MOE_Q_GROUP_128 = 128 };
 MOE_API int moe_add_rmsnorm(float* x_out, const float* x, const float* delta, const moe_bf16_t* weight, int batch, int size, float eps,
                             float* o, moe_bf16_t* o_bf16, uint8_t* q, void* q_scales, int q_group, moe_stream_t stream);

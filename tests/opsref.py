@@ -49,6 +49,14 @@ def rmsnorm(x, w, eps):
     return w.astype(np.float64) * x / np.sqrt((x * x).mean(1, keepdims=True) + np.float64(np.float32(eps)))
 
 
+def rmsnorm_products(x, w, eps):
+    """The same with the steps that moe_rmsnorm takes in fp32: the squares, the mean, its root and the reciprocal; not rounded."""
+    with np.errstate(over="ignore"):
+        mean = (x * x).astype(np.float64).mean(1, keepdims=True) + np.float64(np.float32(eps))
+        inv = np.float32(1) / np.sqrt(mean.astype(np.float32))
+    return w.astype(np.float64) * (inv.astype(np.float64) * x.astype(np.float64))
+
+
 def to_e4m3(v):
     """Nearest e4m3 value (ties to even) of 64-bit numbers up to 448 and a rounding."""
     a = np.abs(v)
@@ -66,27 +74,27 @@ def e4m3_values(codes):
 
 
 def quantise(y, group):
-    """(values code stands for, scales) of fp32 rows y by the rule of moe_add_rmsnorm, the fp32 quotients and products included."""
+    """(values the codes stand for without their scale, scales) of rows y in 64 bits by the rule of moe_add_rmsnorm."""
     B, H = y.shape
     n = H if group == 0 else group
     q, scales = np.zeros((B, H)), np.zeros((B, -(-H // n)))
     for b in range(B):
         for i, k in enumerate(range(0, H, n)):
             v = y[b, k:k + n]
-            if not np.isfinite(v).all():
+            if not np.isfinite(v.astype(np.float32)).all():
                 q[b, k:k + n] = scales[b, i] = np.nan
                 continue
             a = np.abs(v).max()
             if group == 32:
                 p = -126.0
-                while np.float64(a) > 448.0 * 2.0 ** p:
+                while np.float64(np.float32(a)) > 448.0 * 2.0 ** p:
                     p += 1
                 scales[b, i] = 2.0 ** p
-                q[b, k:k + n] = to_e4m3(v.astype(np.float64) / 2.0 ** p)
+                q[b, k:k + n] = to_e4m3(v / 2.0 ** p)
             else:
-                a = np.maximum(a, np.float32(2.0 ** -100))
-                scales[b, i] = a / np.float32(448)
-                q[b, k:k + n] = to_e4m3((v * (np.float32(448) / a)).astype(np.float64))
+                a = np.maximum(a, 2.0 ** -100)
+                scales[b, i] = np.float32(a) / np.float32(448)
+                q[b, k:k + n] = to_e4m3(v / (a / 448.0))
     return q, scales
 
 

@@ -39,7 +39,10 @@ def check(pkg, dev, x, w, group, delta=None, eps=1e-5, in_place=False):
     # relative: fp32 squares and the rounding of their mean, halved by the root: 2^-24; root, quotient and result: half a step each
     assert (np.abs(y - ref) <= 4 * 2.0 ** -24 * np.abs(ref) + 2.0 ** -149).all()
     assert torch.equal(got["o_bf16"], got["o"].bfloat16())
-    wq, ws = opsref.quantise(y, group)
+    # the restatement's sum of squares is the kernel's up to 64-bit roundings, which move the fp32 mean once in 10^8 rows
+    t = opsref.rmsnorm_products(want_x.cpu().numpy(), w.float().cpu().numpy(), eps)
+    assert np.array_equal(t.astype(np.float32), y)
+    wq, ws = opsref.quantise(t, group)
     gs = scales.cpu().numpy()
     gs = np.exp2(gs.astype(np.float64) - 127) if group == 32 else gs.astype(np.float64)
     assert np.array_equal(gs, ws)
@@ -87,11 +90,22 @@ def test_each_output_alone(pkg, dev, H):
 
 
 def test_same_bits_as_rmsnorm(pkg, dev):
-    for H in (64, 1024, 2880):
+    for H in (64, 260, 512, 1024, 1028, 2048, 2880, 4096):
         x, _, w = rows(dev, 9, H, H)
         want = torch.empty_like(x)
         pkg.rmsnorm(want, x, w, 9, H)
         assert torch.equal(call(pkg, dev, x, w, 0)[1]["o"], want)
+
+
+@pytest.mark.parametrize("B,H", [(30000, 1024), (8000, 2880), (3000, 8192), (1500, 16384)])
+def test_rows_past_the_cache(pkg, dev, B, H):
+    """More than 256 MiB of rows take other loads and stores: the bits of parts of the batch."""
+    x, d, w = rows(dev, B, H, H)
+    for group in GROUPS:
+        xo, got, scales = call(pkg, dev, x, w, group, d)
+        for a, b in ((0, 50), (B // 2, B // 2 + 50), (B - 50, B)):
+            po, part, ps = call(pkg, dev, x[a:b].contiguous(), w, group, d[a:b].contiguous())
+            assert torch.equal(po, xo[a:b]) and torch.equal(ps, scales[a:b]) and all(torch.equal(part[k], got[k][a:b]) for k in got)
 
 
 @pytest.mark.parametrize("group", GROUPS)
