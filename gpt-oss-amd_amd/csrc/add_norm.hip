@@ -233,7 +233,7 @@ int launch_add_rmsnorm(const AddNormArgs& a, int batch, hipStream_t stream) {
         if (a.size <= 512) return launch(add_rmsnorm_kernel<64, 2, Q, NT>, 64);
         if (a.size <= 1024) return launch(add_rmsnorm_kernel<64, 4, Q, NT>, 64);
         if (a.size <= 2048) return launch(add_rmsnorm_kernel<256, 2, Q, NT>, 256);
-        if (a.size <= 3072) return launch(add_rmsnorm_kernel<256, 3, Q, NT>, 256);
+        if (a.size <= 3 * 1024) return launch(add_rmsnorm_kernel<256, 3, Q, NT>, 256);
         if (a.size <= 4096) return launch(add_rmsnorm_kernel<256, 4, Q, NT>, 256);
         if (a.size <= 8192) return launch(add_rmsnorm_kernel<512, 4, Q, NT>, 512);
         if (a.size <= 16384) return launch(add_rmsnorm_kernel<1024, 4, Q, NT>, 1024);

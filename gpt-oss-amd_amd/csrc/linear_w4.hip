@@ -9,10 +9,13 @@ namespace moe {
 
 namespace {
 
-constexpr int kUnit = 256;      // contraction elements of a wave: two chunks of 128
+constexpr int kUnit = 256;  // contraction elements of a wave: two chunks of 128
 
 // Waves of a block at most: what the registers of a wave allow (16: 128, 12: 168, 8: 256).
-constexpr int max_waves(int group, int nt) { return group == 32 && nt == 2 ? 8 : nt == 1 && (group == 0 || group == 128) ? 16 : 12; }
+constexpr int max_waves(int group, int nt) {
+    if (group == 32) return nt == 2 ? 8 : 12;
+    return group == 64 && nt == 2 ? 12 : 16;
+}
 
 // e4m3 values times a power of two, to bf16 (exact: three mantissa bits).
 MOE_DEVICE u32x4 e4m3x8_to_bf16(uint32_t lo, uint32_t hi, float scale) {
@@ -33,7 +36,8 @@ __host__ __device__ constexpr int part_floats(int nt, int tiles_per_step) { retu
 // the rate.  Rows past the last and elements past K are zeros (reads past a buffer's end).
 template <int GROUP, int NT>
 MOE_DEVICE void load_x(const LinearArgs& a, uint8_t* bounce, int b0, int u, u32x4 (&xr)[2][4][NT]) {
-    const int lane = threadIdx.x & 63;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // the addresses are made anew for every unit: kept over the loops they cost registers that the weights need
     const int q = lane & 15, g = lane >> 4;
     const uint32_t rows = (uint32_t)min(a.B - b0, 16 * NT), K = (uint32_t)a.K;
     constexpr uint32_t kOutside = 0x80000000u;  // rows * K * 2 < 2^31
@@ -51,15 +55,16 @@ MOE_DEVICE void load_x(const LinearArgs& a, uint8_t* bounce, int b0, int u, u32x
                 for (int n = 0; n < 4; ++n) xr[i][n][t] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)at, (int)((16 * t + 4 * n) * K * 2), 0);
         }
         // piece c (of 16) of row r at position c ^ r of the row's 256 bytes: no two lanes of a read meet in a bank
+        const uint32_t put = g * 256 + ((q ^ g) << 4), get = q * 256 + ((GROUP ? g ^ q : 4 * g ^ q) << 4);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int n = 0; n < 4; ++n) *reinterpret_cast<u32x4*>(bounce + (4 * n + g) * 256 + ((q ^ (4 * n + g)) << 4)) = xr[i][n][t];
+                for (int n = 0; n < 4; ++n) *reinterpret_cast<u32x4*>(bounce + 1024 * n + (put ^ (n << 6))) = xr[i][n][t];  // row 4n + g, piece q
                 lds_in_order();
 #pragma unroll
-                for (int j = 0; j < 4; ++j) xr[i][j][t] = *reinterpret_cast<const u32x4*>(bounce + q * 256 + (((GROUP ? 4 * j + g : 4 * g + j) ^ q) << 4));
+                for (int j = 0; j < 4; ++j) xr[i][j][t] = *reinterpret_cast<const u32x4*>(bounce + (get ^ (GROUP ? j << 6 : j << 4)));  // 4j + g : 4g + j
                 lds_in_order();
             }
     } else {
@@ -68,6 +73,8 @@ MOE_DEVICE void load_x(const LinearArgs& a, uint8_t* bounce, int b0, int u, u32x
         const __amdgpu_buffer_rsrc_t s_rsrc = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<uint8_t*>(a.x_scales + (size_t)b0 * (K / 32)), 0, (int)(rows * (K / 32)), 0x00020000);
         // eight rows of 128 bytes to an instruction; the scale of the lane's row q and 32 elements g
+        const uint32_t put = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 4)) << 4);
+        const uint32_t get = GROUP ? q * 128 + (((g ^ q) >> 1) << 4) + 8 * (g & 1) : q * 128 + ((2 * g ^ q >> 1) << 4);
         u32x4 c[2][2][NT];
         uint32_t s[2][NT];
 #pragma unroll
@@ -87,15 +94,12 @@ MOE_DEVICE void load_x(const LinearArgs& a, uint8_t* bounce, int b0, int u, u32x
             for (int i = 0; i < 2; ++i) {
                 // piece p (of 8) of row r at position p ^ (r / 2) of the row's 128 bytes
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const int r = 8 * n + (lane >> 3);
-                    *reinterpret_cast<u32x4*>(bounce + r * 128 + (((lane & 7) ^ (r >> 1)) << 4)) = c[i][n][t];
-                }
+                for (int n = 0; n < 2; ++n) *reinterpret_cast<u32x4*>(bounce + 1024 * n + (put ^ (n << 6))) = c[i][n][t];  // row 8n + lane / 8
                 lds_in_order();
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int e = GROUP ? 32 * j + 8 * g : 32 * g + 8 * j;  // of 128, a byte each
-                    const uint2 v = *reinterpret_cast<const uint2*>(bounce + q * 128 + (((e >> 4) ^ (q >> 1)) << 4) + (e & 8));
+                    // bytes 32 j + 8 g .. of the row's 128 : 32 g + 8 j
+                    const uint2 v = *reinterpret_cast<const uint2*>(bounce + (GROUP ? get ^ (j << 5) : (get ^ (j >> 1 << 4)) + 8 * (j & 1)));
                     const uint32_t sb = GROUP ? (uint32_t)__shfl((int)s[i][t], 16 * j + q) : s[i][t];
                     xr[i][j][t] = e4m3x8_to_bf16(v.x, v.y, mxfp4_scale_to_f32(sb));
                 }
@@ -278,26 +282,35 @@ __global__ __launch_bounds__(64 * max_waves(GROUP, NT)) void linear_tile_kernel(
     }
 }
 
+// Waves of a block of linear_w4_kernel that add up what the others leave: one for each tile of 16 x 16 of a step, up to a quarter of all.
+constexpr int adders(int group, int nt, int tiles_per_step) {
+    const int most = max_waves(group, nt) / 4;
+    return nt * tiles_per_step < most ? nt * tiles_per_step : most;
+}
+
 // How a launch is cut: a block has wk x wr waves; the contraction's units are dealt out over wk waves, in as many slabs as that takes, and its
 // tiles of 16 weight rows, tiles_per_block consecutive ones, over wr.
 struct LinearCut {
     int wk, log_wr, n_slabs, tiles_per_block;
+    int inv_wk;  // 65536 / wk, rounded up
     int tiles_per_step;  // tile sets between two barriers that there is room for
 };
 
 // GROUP 0: MXFP4 weights in the tiled layout of mxfp4.hip; else int4 codes with a scale per GROUP values (layout of int4_repack_kernel).
-// A wave holds its unit of 16 NT rows of x in registers and goes through the block's tiles, the weights of the next D in flight; the waves of
-// a tile meet in LDS and one of them, another for every tile, adds up.  A result is the sum over units in ascending order, whatever the
-// cut: it does not depend on how many rows x has.
+// A wave holds its unit of 16 NT rows of x in registers and goes through the block's tiles, the weights of the next D in flight; every G tiles
+// the waves meet, and further waves add up the partial tiles that they have left in LDS, while they go on.  A result is the sum over units in
+// ascending order, whatever the cut: it does not depend on how many rows x has.
 template <int GROUP, int NT, int D, int G>
 __global__ __launch_bounds__(64 * max_waves(GROUP, NT)) void linear_w4_kernel(LinearArgs a, LinearCut cut) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
-    constexpr int kPart = NT * 256;                     // values of a tile
+    constexpr int kPart = NT * 256;  // values of a tile
+    constexpr int kAdders = adders(GROUP, NT, G);
     // grid (8, token blocks, tile blocks / 8): token blocks of the same weights side by side on one XCD; no quotient is formed in here, each is
     // a chain of forty instructions, and a launch for one row is little more than a few chains
     const int lane = threadIdx.x & 63;
-    const int wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = __builtin_amdgcn_readfirstlane(threadIdx.y);
-    const int n_wr = 1 << cut.log_wr, waves = cut.wk << cut.log_wr, wave = wr * cut.wk + wk;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n_wr = 1 << cut.log_wr, waves = cut.wk << cut.log_wr;  // and kAdders more
+    const int wr = wave * cut.inv_wk >> 16, wk = wave - wr * cut.wk;
     const int q = lane & 15, g = lane >> 4;
     const int n_units = ceil_div(a.K, kUnit);
     const int n_tiles = ceil_div(a.N, 16);
@@ -312,79 +325,96 @@ __global__ __launch_bounds__(64 * max_waves(GROUP, NT)) void linear_w4_kernel(Li
     float* const sums = bias + cut.tiles_per_block * 16;    // [tiles_per_block][kPart] between slabs
     const int b0 = token_block * 16 * NT;
     const int n_bias = (tile1 - tile0) * 16;
-    for (int i = 64 * wave + lane; i < n_bias; i += 64 * waves) {
+    for (int i = threadIdx.x; i < n_bias; i += 64 * (waves + kAdders)) {
         const int n = weight_row<GROUP>(tile0 + (i >> 4), i & 15);
         bias[i] = a.bias && n < a.N ? bf16_bits_to_f32(a.bias[n]) : 0.f;
     }
-    UnitWeights<GROUP> w[D];
+    // The block's sets of n_wr tiles; blocks begin at different ones of theirs: side by side they would read from the same few channels of the
+    // memory (1 row of 131072 x 2880 34.4 : 33.5 us, 16 rows of 262144 x 2880 78.1 : 74.6).  Not with more rows, where blocks with the same
+    // tiles run beside each other (64 rows of 131072 x 2880 62.8 : 64.2).
+    const int n_sets = (tile1 - tile0 + n_wr - 1) >> cut.log_wr;
+    const int first_set = NT == 1 ? (n_sets * (tile_block & 31) >> 5) & -G : 0;
+    auto first_tile = [&](int j) {
+        const int set = j + first_set;
+        return tile0 + ((set >= n_sets ? set - n_sets : set) << cut.log_wr);
+    };
+    constexpr int kPass = D > G ? D : G;
+    int half = 0;  // which half of `part` a step writes
 
-    int half = 0, turn = 0;  // which half of `part` a step writes, and which wave adds up its first item
+    if (wave >= waves) {
+        // The waves that add up.  They load nothing: a wave's loads and stores are waited for in their order, and a store in front of the next
+        // weights holds up the wave, and all others at the next meeting (131072 x 2880, by the waves themselves : by these, 16 rows 39.4 : 38.4 us,
+        // 64 rows 72 : 63).
+        for (int slab = 0; slab < n_slabs; ++slab) {
+            const int units = min(cut.wk, n_units - slab * cut.wk);
+            for (int j = 0; j < (n_sets + kPass - 1) / kPass * kPass; j += G) {
+                __syncthreads();
+                // item (m, w, t): token tile t of the m-th tile of row wave w
+                const int items = (max(0, min(G, n_sets - j)) << cut.log_wr) * NT;
+                for (int item = wave - waves; item < items; item += kAdders) {
+                    const int set = item / NT, t = item - set * NT;
+                    const int m = set >> cut.log_wr, w = set & (n_wr - 1);
+                    const int tl = first_tile(j + m) + w;  // wave-uniform
+                    if (tl >= tile1) continue;
+                    const float* src = part + w * cut.wk * per_wave + (half * cut.tiles_per_step + m) * kPart + t * 256 + lane * 4;
+                    float* const between = sums + (tl - tile0) * kPart + t * 256 + lane * 4;
+                    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                    if (slab > 0) v = *reinterpret_cast<const f32x4*>(between);
+#pragma unroll 4
+                    for (int i = 0; i < units; ++i) v += *reinterpret_cast<const f32x4*>(src + i * per_wave);
+                    if (slab + 1 < n_slabs) {
+                        *reinterpret_cast<f32x4*>(between) = v;
+                        continue;
+                    }
+                    const int b = b0 + t * 16 + q;
+                    v += *reinterpret_cast<const f32x4*>(bias + (tl - tile0) * 16 + 4 * g);
+                    if (b < a.B) store_results(a, b, weight_row<GROUP>(tl, 4 * g), v);
+                }
+                half ^= 1;
+            }
+            if (slab + 1 < n_slabs) __syncthreads();
+        }
+        return;
+    }
+
+    UnitWeights<GROUP> w[D];
     for (int slab = 0; slab < n_slabs; ++slab) {
         const int u = slab * cut.wk + wk;
-        auto load_slot = [&](int d, int tile) { w[d].load(a, min(tile, n_tiles - 1), u, tile < tile1 && u < n_units); };
-        load_slot(0, tile0 + wr);
+        auto load_slot = [&](int d, int j) {
+            const int tile = first_tile(j) + wr;
+            w[d].load(a, min(tile, n_tiles - 1), u, j < n_sets && tile < tile1 && u < n_units);
+        };
+        load_slot(0, 0);
         u32x4 xr[2][4][NT];
         load_x<GROUP, NT>(a, reinterpret_cast<uint8_t*>(part + wave * per_wave), b0, u, xr);
         __builtin_amdgcn_sched_barrier(0);  // the other slots' registers are free until x is where it stays
 #pragma unroll
-        for (int d = 1; d < D; ++d) load_slot(d, tile0 + wr + d * n_wr);
+        for (int d = 1; d < D; ++d) load_slot(d, d);
         float sum_x[UnitWeights<GROUP>::kGroups][NT];
         group_sums<GROUP, NT>(xr, sum_x);
-        // partial tile of slot S of the ring, the M-th of its step
-        auto tile_part = [&](auto slot_tag, int m, int tile) {
+        // partial tile of set j, in slot S of the ring, the m-th of its step
+        auto tile_part = [&](auto slot_tag, int m, int j) {
             constexpr int S = decltype(slot_tag)::value;
             f32x4 acc[NT];
             w[S].template multiply<NT>(a.w_zeros != nullptr, u, xr, sum_x, acc);
             __builtin_amdgcn_sched_barrier(0);
-            load_slot(S, tile + D * n_wr);  // the slot is free
+            load_slot(S, j + D);  // the slot is free
             __builtin_amdgcn_sched_barrier(0);
-            if (tile - wr >= tile1) return;  // a set that is not this block's: block-uniform
+            if (j >= n_sets) return;  // block-uniform
             float* const mine = part + wave * per_wave + ((half * cut.tiles_per_step) + m) * kPart;
 #pragma unroll
             for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(mine + t * 256 + lane * 4) = acc[t];
         };
-        // The G tile sets from `tile` on: item (m, w, t), token tile t of the m-th tile of row wave w, is added up by one wave; the items of
-        // the steps go round over the waves.
-        auto add_up = [&](int tile) {
-            __syncthreads();
-            const int units = min(cut.wk, n_units - slab * cut.wk);
-            const int items = max(0, min(G << cut.log_wr, tile1 - tile)) * NT;
-            auto add = [&](int item) {
-                const int set = item / NT, t = item - set * NT;
-                const int m = set >> cut.log_wr, w = set & (n_wr - 1);
-                const int tl = tile + set;  // wave-uniform
-                const float* src = part + w * cut.wk * per_wave + (half * cut.tiles_per_step + m) * kPart + t * 256 + lane * 4;
-                float* const between = sums + (tl - tile0) * kPart + t * 256 + lane * 4;
-                f32x4 v = {0.f, 0.f, 0.f, 0.f};
-                if (slab > 0) v = *reinterpret_cast<const f32x4*>(between);
-#pragma unroll 4
-                for (int i = 0; i < units; ++i) v += *reinterpret_cast<const f32x4*>(src + i * per_wave);
-                if (slab + 1 < n_slabs) {
-                    *reinterpret_cast<f32x4*>(between) = v;
-                    return;
-                }
-                const int b = b0 + t * 16 + q;
-                if (b >= a.B) return;
-                v += *reinterpret_cast<const f32x4*>(bias + (tl - tile0) * 16 + 4 * g);
-                store_results(a, b, weight_row<GROUP>(tl, 4 * g), v);
-            };
-            // without a loop where one round does: in front of a loop that stores, the compiler waits for every load in flight
-            int item = wave - turn;
-            if (item < 0) item += waves;
-            if (item < items) add(item);
-            if (items > waves)
-                for (item += waves; item < items; item += waves) add(item);
-            turn += items;
-            while (turn >= waves) turn -= waves;
-            half ^= 1;
-        };
-        // the ring's slots are constants: D or G tile sets, whichever is more, to a pass of the loop
-        for (int tile = tile0; tile < tile1; tile += (D > G ? D : G) * n_wr) {
+        // the ring's slots are constants: D or G sets, whichever is more, to a pass of the loop
+        for (int j = 0; j < n_sets; j += kPass) {
             auto at = [&](auto m_tag) {
                 constexpr int M = decltype(m_tag)::value;
-                if constexpr (M < (D > G ? D : G)) {
-                    tile_part(std::integral_constant<int, M % D>{}, M % G, tile + M * n_wr + wr);
-                    if constexpr (M % G == G - 1) add_up(tile + (M - G + 1) * n_wr);
+                if constexpr (M < kPass) {
+                    tile_part(std::integral_constant<int, M % D>{}, M % G, j + M);
+                    if constexpr (M % G == G - 1) {
+                        __syncthreads();
+                        half ^= 1;
+                    }
                 }
             };
             at(std::integral_constant<int, 0>{});
@@ -415,19 +445,22 @@ template <int GROUP, int NT, int D, int G>
 static int launch_linear_of(const LinearArgs& a, int n_cus, hipStream_t stream) {
     const int n_tiles = ceil_div(a.N, 16), n_units = ceil_div(a.K, kUnit);
     LinearCut cut;
-    const int slabs = ceil_div(n_units, max_waves(GROUP, NT));
+    constexpr int kAdders = adders(GROUP, NT, G);
+    const int slabs = ceil_div(n_units, max_waves(GROUP, NT) - kAdders);
     cut.n_slabs = slabs;
     cut.wk = ceil_div(n_units, slabs);
+    cut.inv_wk = ceil_div(65536, cut.wk);
     cut.log_wr = 0;
-    while (cut.wk << (cut.log_wr + 1) <= 8 && n_tiles >> cut.log_wr > n_cus) ++cut.log_wr;
+    while ((cut.wk << (cut.log_wr + 1)) + kAdders <= std::min(12, max_waves(GROUP, NT)) && n_tiles >> cut.log_wr > n_cus) ++cut.log_wr;
     const int wr = 1 << cut.log_wr, waves = cut.wk * wr, token_blocks = ceil_div(a.B, 16 * NT);
-    const int at_once = n_cus * std::max(1, max_waves(GROUP, NT) / waves);
+    const int at_once = n_cus * std::max(1, max_waves(GROUP, NT) / (waves + kAdders));
     const int most = (slabs > 1 ? 32 / NT : 128) / wr;  // what the LDS has room for
     cut.tiles_per_block = std::min(most, ceil_div(n_tiles * token_blocks, at_once * wr)) * wr;
     cut.tiles_per_step = std::min(G, cut.tiles_per_block / wr);
     const size_t lds = (size_t)waves * part_floats(NT, cut.tiles_per_step) * 4 + (size_t)cut.tiles_per_block * (64 + (slabs > 1 ? NT * 1024 : 0));
     const int blocks = ceil_div(n_tiles, cut.tiles_per_block);
-    hipLaunchKernelGGL((linear_w4_kernel<GROUP, NT, D, G>), dim3(8, token_blocks, ceil_div(blocks, 8)), dim3(64 * cut.wk, wr), lds, stream, a, cut);
+    hipLaunchKernelGGL((linear_w4_kernel<GROUP, NT, D, G>), dim3(8, token_blocks, ceil_div(blocks, 8)), dim3(64 * (waves + kAdders)), lds,
+                       stream, a, cut);
     return launch_status();
 }
 
@@ -437,9 +470,9 @@ static int launch_linear_rows(const LinearArgs& a, int n_cus, hipStream_t stream
     const int n_units = ceil_div(a.K, kUnit);
     const long long tiles = (long long)ceil_div(a.N, 16) * ceil_div(a.B, 16 * NT);
     if (tiles <= n_cus && linear_tile_lds(GROUP, NT, n_units) <= kLdsMost) return launch_linear_tile<GROUP, NT>(a, n_units, stream);
-    // with three tiles to a block the ring and the shared steps of the second form cost more code than they hide: us, first : second form, 1 row of
-    // 5760 x 2880 MXFP4 5.8 : 6.5, 16 rows of 16384 x 4096 11.9 : 11.2, of 131072 x 2880 45.7 : 38.9; more than 128 int4 scales a block of weights
-    // do not fit its registers: scales per 64, 32 rows, and per 32
+    // With up to three tiles to a block the longer ring and the wider steps of the second form cost more code than they hide: us, first : second
+    // form, 1 row of 5760 x 2880 MXFP4 5.8 : 6.2, 7 rows with int4 scales per 64 7.1 : 8.5, 1 row of 16384 x 4096 MXFP4 11.7 : 10.1, 16 rows of
+    // 131072 x 2880 42.7 : 38.6.  More than 128 int4 scales to a tile's unit, those per 64 with 32 rows and those per 32, do not fit a ring of two.
     if (tiles <= 3LL * n_cus || GROUP == 32 || (GROUP == 64 && NT == 2)) return launch_linear_of<GROUP, NT, 1, 2>(a, n_cus, stream);
     if constexpr (!(GROUP == 32 || (GROUP == 64 && NT == 2))) return launch_linear_of<GROUP, NT, 2, 4 / NT>(a, n_cus, stream);
     return MOE_ERR_LIMIT;
