@@ -276,6 +276,9 @@ int moe_softmax(float* x, int batch_size, int size, moe_stream_t stream) {
     return launch_softmax_rows(x, batch_size, size, as_stream(stream));
 }
 
+// Rows that share blocks are counted in 32 bits, the last block's beyond the last row too.
+constexpr int kMostRows = 0x7FFFFF00;
+
 static int check_route(const moe_route_params* rule, int E, int K) {
     if (rule->struct_bytes != sizeof(moe_route_params)) return MOE_ERR_FORMAT;
     if (rule->scoring != MOE_ROUTE_SOFTMAX && rule->scoring != MOE_ROUTE_SIGMOID) return MOE_ERR_FORMAT;
@@ -296,6 +299,7 @@ int moe_route(float* topk_values, int* topk_indices, const float* router_logits,
               int experts_per_token, const moe_route_params* rule, moe_stream_t stream) {
     if (!topk_values || !topk_indices || !router_logits || !rule) return MOE_ERR_NULL;
     if (batch_size <= 0) return MOE_ERR_SHAPE;
+    if (batch_size > kMostRows) return MOE_ERR_LIMIT;
     const int rc = check_route(rule, num_experts, experts_per_token);
     if (rc) return rc;
     return launch_route(router_logits, topk_values, topk_indices, batch_size, num_experts, experts_per_token, route_rule(rule),
@@ -529,6 +533,7 @@ int moe_add_rmsnorm(float* x_out, const float* x, const float* delta, const moe_
                     float* o, moe_bf16_t* o_bf16, uint8_t* q, void* q_scales, int q_group, moe_stream_t stream) {
     if (!x_out || !x || !weight || (!o && !o_bf16 && !q) || (q != nullptr) != (q_scales != nullptr)) return MOE_ERR_NULL;
     if (batch <= 0 || size <= 0 || size % 4 != 0) return MOE_ERR_SHAPE;
+    if (batch > kMostRows) return MOE_ERR_LIMIT;
     if (q && q_group != MOE_Q_GROUP_ROW && q_group != MOE_Q_GROUP_MX && q_group != MOE_Q_GROUP_128) return MOE_ERR_FORMAT;
     if (q && q_group == MOE_Q_GROUP_MX && size % 32 != 0) return MOE_ERR_SHAPE;
     if (((uintptr_t)x_out | (uintptr_t)x | (uintptr_t)delta | (uintptr_t)o) & 15u) return MOE_ERR_ALIGN;
@@ -542,7 +547,7 @@ int moe_add_rmsnorm(float* x_out, const float* x, const float* delta, const moe_
 static int check_linear(const void* y, const void* x, const void* w, const void* w_scales, const void* bias, int B, int K, int N) {
     if (!y || !x || !w || !w_scales) return MOE_ERR_NULL;
     if (B <= 0 || K <= 0 || N <= 0 || K % 32 != 0) return MOE_ERR_SHAPE;
-    if (B > 65535 || K > (1 << 24)) return MOE_ERR_LIMIT;
+    if (B > 65535 || K > (1 << 24) || N > (1 << 26)) return MOE_ERR_LIMIT;  // N: blocks of at least 16 tiles, 8 * 65535 of them
     if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)w_scales) & 15u) return MOE_ERR_ALIGN;
     if (((uintptr_t)y & 3u) || ((uintptr_t)bias & 1u)) return MOE_ERR_ALIGN;
     return MOE_OK;

@@ -2,7 +2,8 @@
 // fp64, sqrtf and the reciprocal in fp32, the scaling in fp64, one rounding to fp32 at the end.
 // A row is owned by one block of 256 threads; thread i holds float4 columns i, i + 256, ... and adds
 // their squares in ascending order, the fp64 sum over the block is a fixed tree over each wave and then the waves in order: results
-// are run-to-run identical, and identical between the plain kernel and the ones fused into the combine and the residual add.
+// are run-to-run identical, and identical between the plain kernel, the one fused into the combine and, for rows of up to 4096 values, the
+// one with the residual add (longer rows take more threads there, so another order of the fp64 sum).
 #pragma once
 #include "common.h"
 

@@ -131,8 +131,8 @@ MOE_API int moe_softmax(float* x, int batch_size, int size, moe_stream_t stream)
  *   chosen    : the experts_per_token largest choices of the groups that stay, in descending order, equal ones: the lower index.  A NaN
  *               counts as +infinity, a group's value too.  The indices of a token are distinct and in range whatever its logits hold
  *   value     = score[chosen], divided by the sum over the chosen if renormalize (0 where that sum is 0), times scale (fp64, rounded once)
- * num_experts <= 1024, a multiple of n_groups; n_groups <= 64; experts_per_token <= 8 and <= the experts of the groups that stay.  The
- * rule is host memory, read during the call; balance_bias [num_experts] is device memory or NULL. */
+ * batch_size < 2^31 - 255; num_experts <= 1024, a multiple of n_groups; n_groups <= 64; experts_per_token <= 8 and <= the experts of
+ * the groups that stay.  The rule is host memory, read during the call; balance_bias [num_experts] is device memory or NULL. */
 enum { MOE_ROUTE_SOFTMAX = 0, MOE_ROUTE_SIGMOID = 1 };
 typedef struct moe_route_params {
     uint32_t struct_bytes;    /* sizeof(moe_route_params) of the caller's header */
@@ -286,7 +286,7 @@ MOE_API int moe_rmsnorm(float* o, const float* x, const moe_bf16_t* weight, int 
  *   q_group 128  the largest |y| of the group, 2^-100 at least, over 448; the last group may be shorter.  Scales fp32
  *                [batch, ceil(size / 128)]: that |y| in fp32, divided in fp32.  q_group 0 the same with one group a row, scales [batch]
  * A group that holds an infinity or a NaN has a NaN for its scale and for every code.  x_out may be x; otherwise no output may overlap an
- * input.  size % 4 == 0; x, x_out, delta and o 16-byte aligned, weight and o_bf16 8-byte, q and fp32 scales 4-byte. */
+ * input.  size % 4 == 0, batch < 2^31 - 255; x, x_out, delta and o 16-byte aligned, weight and o_bf16 8-byte, q and fp32 scales 4-byte. */
 enum { MOE_Q_GROUP_ROW = 0, MOE_Q_GROUP_MX = 32, MOE_Q_GROUP_128 = 128 };
 MOE_API int moe_add_rmsnorm(float* x_out, const float* x, const float* delta, const moe_bf16_t* weight, int batch, int size, float eps,
                             float* o, moe_bf16_t* o_bf16, uint8_t* q, void* q_scales, int q_group, moe_stream_t stream);
@@ -298,7 +298,8 @@ MOE_API int moe_add_rmsnorm(float* x_out, const float* x, const float* delta, co
 
 /* y[b, n] = bias[n] + sum_k x[b, k] W[n, k], fp32 sums, for B rows and an N x K matrix; made for decode-sized batches (the weights are read
  * once per 64 rows).  x [B, K] is bf16 (x_scales NULL) or e4m3 codes with x_scales [B, K / 32] e8m0 as moe_add_rmsnorm writes them (byte 0
- * counts as a factor of 0, as in weights).  bias [N] bf16 or NULL.  K % 32 == 0, K <= 2^24, B <= 65535; x and the tiled tensors 16-byte aligned.
+ * counts as a factor of 0, as in weights).  bias [N] bf16 or NULL.  K % 32 == 0, K <= 2^24, N <= 2^26, B <= 65535; x and the tiled tensors 16-byte
+ * aligned.
  * Deterministic, and a row's result does not depend on the rows around it.
  *
  * moe_linear_mxfp4: tiled_blocks / tiled_scales of moe_mxfp4_repack(E = 1, rows = N, K); N % 64 == 0.

@@ -19,6 +19,7 @@ def test_route_refuses(pkg):
     assert f(None, 16, 16, 4, 32, 4, rule(pkg), None) == f(16, 16, 16, 4, 32, 4, None, None) == -1
     assert f(16, 16, 16, 0, 32, 4, rule(pkg), None) == f(16, 16, 16, 4, 3, 4, rule(pkg), None) == f(16, 16, 16, 4, 32, 0, rule(pkg), None) == -2
     assert f(16, 16, 16, 4, 1025, 4, rule(pkg), None) == f(16, 16, 16, 4, 32, 9, rule(pkg), None) == -3
+    assert f(16, 16, 16, 0x7FFFFF01, 1, 1, rule(pkg), None) == -3
     assert f(16, 16, 16, 4, 520, 4, rule(pkg, n_groups=65, groups_per_token=4), None) == -3
     assert f(16, 16, 16, 4, 32, 4, rule(pkg, scoring=2), None) == f(16, 16, 16, 4, 32, 4, rule(pkg, struct_bytes=8), None) == -5
     for bad in (dict(n_groups=0), dict(n_groups=5), dict(n_groups=4, groups_per_token=0), dict(n_groups=4, groups_per_token=5), dict(group_top=0),
@@ -57,6 +58,7 @@ def test_add_rmsnorm_refuses(pkg):
         return f(a["x_out"], a["x"], a["delta"], a["w"], a["batch"], a["size"], a["eps"], a["o"], a["ob"], a["q"], a["qs"], a["group"], None)
     assert call(x_out=None) == call(x=None) == call(w=None) == call(q=None) == call(qs=None) == call(o=None, ob=None, q=None, qs=None) == -1
     assert call(batch=0) == call(size=0) == call(size=66) == call(size=68) == -2  # the last: no multiple of 32 for scales of 32
+    assert call(batch=0x7FFFFF01, size=4, group=0) == -3
     assert call(group=64) == -5
     assert call(x=8) == call(x_out=8) == call(delta=4) == call(o=8) == call(w=4) == call(ob=4) == call(q=2) == call(qs=2, group=0) == -6
 
@@ -66,7 +68,7 @@ def test_linear_refuses(pkg):
     assert f(None, 16, None, 16, 16, None, 1, 64, 64, None) == f(16, 16, None, 16, None, None, 1, 64, 64, None) == -1
     assert f(16, 16, None, 16, 16, None, 0, 64, 64, None) == f(16, 16, None, 16, 16, None, 1, 48, 64, None) == -2
     assert f(16, 16, None, 16, 16, None, 1, 64, 32, None) == -2  # rows of tiled MXFP4 come in groups of 64
-    assert f(16, 16, None, 16, 16, None, 65536, 64, 64, None) == -3
+    assert f(16, 16, None, 16, 16, None, 65536, 64, 64, None) == f(16, 16, None, 16, 16, None, 1, 64, 2**26 + 64, None) == -3
     assert f(16, 8, None, 16, 16, None, 1, 64, 64, None) == f(2, 16, None, 16, 16, None, 1, 64, 64, None) == f(16, 16, None, 16, 16, 1, 1, 64, 64, None) == -6
     assert g(16, None, None, 16, 16, None, None, 1, 64, 5, 32, None) == -1
     assert g(16, 16, None, 16, 16, None, None, 1, 64, 0, 32, None) == -2
