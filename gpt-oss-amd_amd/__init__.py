@@ -176,10 +176,13 @@ def _ptr(t):
     return t.data_ptr()
 
 
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _device():
     """Index of the current device; without one an index that no tensor has."""
     try:
-        return torch._C._cuda_getDevice()
+        return _current_device()
     except RuntimeError:
         return -2
 
@@ -198,9 +201,9 @@ def _arg(name, t, dtype, n, dev):
 
 
 # torch.cuda.current_stream() makes a stream object on every call: 2.9 us, as much as a launch; the handle alone 0.2
-def _stream(stream):
+def _stream(stream, dev=None):
     if stream is None:
-        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+        return _raw_stream(_current_device() if dev is None else dev)
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
 
 
@@ -269,7 +272,7 @@ def route(topk_values, topk_indices, router_logits, batch_size, num_experts, exp
     n, dev = batch_size * experts_per_token, _device()
     rc = _lib.moe_route(_arg("topk_values", topk_values, _f32, n, dev), _arg("topk_indices", topk_indices, torch.int32, n, dev),
                         _arg("router_logits", router_logits, _f32, batch_size * num_experts, dev), batch_size, num_experts,
-                        experts_per_token, rule.of(num_experts), _stream(stream))
+                        experts_per_token, rule.of(num_experts), _stream(stream, dev))
     if rc:
         raise MoeError("moe_route", rc)
 
@@ -391,7 +394,7 @@ def add_rmsnorm(x_out, x, weight, batch, size, delta=None, eps=1e-5, o=None, o_b
     rc = _lib.moe_add_rmsnorm(_arg("x_out", x_out, _f32, n, dev), _arg("x", x, _f32, n, dev), _arg("delta", delta, _f32, n, dev),
                               _arg("weight", weight, _bf16, size, dev), batch, size, eps, _arg("o", o, _f32, n, dev),
                               _arg("o_bf16", o_bf16, _bf16, n, dev), _arg("q", q, _u8, n, dev),
-                              _arg("q_scales", q_scales, _u8 if q_group == MOE_Q_GROUP_MX else _f32, n_scales, dev), q_group, _stream(stream))
+                              _arg("q_scales", q_scales, _u8 if q_group == MOE_Q_GROUP_MX else _f32, n_scales, dev), q_group, _stream(stream, dev))
     if rc:
         raise MoeError("moe_add_rmsnorm", rc)
 
@@ -410,7 +413,7 @@ def linear_mxfp4(y, x, tiled_blocks, tiled_scales, B, K, N, bias=None, x_scales=
     xp, xs = _linear_rows(x, x_scales, B, K, dev)
     rc = _lib.moe_linear_mxfp4(_arg("y", y, _f32, B * N, dev), xp, xs, _arg("tiled_blocks", tiled_blocks, _u8, N * K // 2, dev),
                                _arg("tiled_scales", tiled_scales, _u8, N * (-(-K // 512) * 16), dev), _arg("bias", bias, _bf16, N, dev),
-                               B, K, N, _stream(stream))
+                               B, K, N, _stream(stream, dev))
     if rc:
         raise MoeError("moe_linear_mxfp4", rc)
 
@@ -447,7 +450,7 @@ def linear_int4(y, x, tiled_codes, tiled_scales, B, K, N, group, tiled_zeros=Non
     n = rows * (-(-K // 256) * 256 // group) if group > 0 else 0
     rc = _lib.moe_linear_int4(_arg("y", y, _f32, B * N, dev), xp, xs, _arg("tiled_codes", tiled_codes, _u8, rows * (-(-K // 128) * 64), dev),
                               _arg("tiled_scales", tiled_scales, _bf16, n, dev), _arg("tiled_zeros", tiled_zeros, _u8, n, dev),
-                              _arg("bias", bias, _bf16, N, dev), B, K, N, group, _stream(stream))
+                              _arg("bias", bias, _bf16, N, dev), B, K, N, group, _stream(stream, dev))
     if rc:
         raise MoeError("moe_linear_int4", rc)
 
