@@ -33,15 +33,27 @@ __host__ __device__ constexpr int part_floats(int nt, int tiles_per_step) { retu
 // Unit u of rows b0 .. b0 + 16 NT - 1 of x, as xr[chunk][MFMA step][token tile]: token q, 8 elements per lane, which are 32 g + 8 j .. of the chunk
 // for MXFP4 weights and 32 j + 8 g .. for int4.  Loaded in whole lines, 16 bytes of consecutive lanes side by side, and brought to the
 // lanes that need them through `bounce`, 4 KiB of LDS of this wave alone: loads whose lanes follow the operand layout run at a quarter of
-// the rate.  Rows past the last and elements past K are zeros (reads past a buffer's end).
-template <int GROUP, int NT>
-MOE_DEVICE void load_x(const LinearArgs& a, uint8_t* bounce, int b0, int u, u32x4 (&xr)[2][4][NT]) {
+// the rate.  Those of one row do not and go without (2880 x 2880, through LDS : without, 1 row 4.29 : 4.15 us, 4 rows 4.41 : 4.59, 16 rows 4.88 : 6.25).
+// Rows past the last and elements past K are zeros (reads past a buffer's end).
+enum RowForm { kRowsBf16, kRowsE4m3, kOneRowBf16 };
+template <int GROUP, int NT, int FORM>
+MOE_DEVICE void load_x(const LinearArgs& a, [[maybe_unused]] uint8_t* bounce, int b0, int u, u32x4 (&xr)[2][4][NT]) {
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));  // the addresses are made anew for every unit: kept over the loops they cost registers that the weights need
     const int q = lane & 15, g = lane >> 4;
     const uint32_t rows = (uint32_t)min(a.B - b0, 16 * NT), K = (uint32_t)a.K;
     constexpr uint32_t kOutside = 0x80000000u;  // rows * K * 2 < 2^31
-    if (a.x_scales == nullptr) {
+    if constexpr (FORM == kOneRowBf16) {
+        static_assert(NT == 1);
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.x), 0, (int)(K * 2), 0x00020000);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t k = kUnit * u + 128 * i + (GROUP ? 32 * j + 8 * g : 32 * g + 8 * j);
+                xr[i][j][0] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(q == 0 ? k * 2 : kOutside), 0, 0);
+            }
+    } else if constexpr (FORM == kRowsBf16) {
         const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<uint16_t*>(static_cast<const uint16_t*>(a.x) + (size_t)b0 * K), 0, (int)(rows * K * 2), 0x00020000);
         // four rows of 256 bytes to an instruction
@@ -245,10 +257,10 @@ MOE_DEVICE f32x4 load_bias(const LinearArgs& a, int n) {  // 0 without one, and 
 }
 
 // Few tiles: a block for each, its waves take the units in turn.  Such a launch is a chain of latencies (arguments, weights and rows, LDS
-// and back, the waves' meeting, stores), so its code is short and nothing waits before the first loads are out.  ONE: a wave to every unit, and no loop
-// over them (1 row of 2880 x 2880 4.43 : 4.29 us, 16 rows 4.93 : 4.72).  In the loop nothing is loaded ahead: with the next unit's weights on their way 4
-// rows of 4096 x 16384 took 13.7 : 13.3 us, but 40 rows of 4096 x 8192 15.6 : 16.0, and its rows as well did not fit the registers.
-template <int GROUP, int NT, bool ONE>
+// and back, the waves' meeting, stores), so its code is short and nothing waits before the first loads are out: kernels of their own for each form of
+// x and (ONE) for a wave to every unit, without a loop over them.  All in one : so, us: 1 row of 2880 x 2880 4.43 : 3.96, 16 rows 4.93 : 4.78, 1 row of
+// 2880 x 8192 7.5 : 7.0.  In the loop nothing is loaded ahead: with the next unit's weights on their way 1 row of 4096 x 16384 took 11.7 : 12.0.
+template <int GROUP, int NT, int FORM, bool ONE>
 __global__ __launch_bounds__(64 * max_waves(GROUP, NT)) void linear_tile_kernel(LinearArgs a) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int lane = threadIdx.x & 63;
@@ -263,7 +275,7 @@ __global__ __launch_bounds__(64 * max_waves(GROUP, NT)) void linear_tile_kernel(
         UnitWeights<GROUP> w;
         w.load(a, tile, u, true);
         u32x4 xr[2][4][NT];
-        load_x<GROUP, NT>(a, bounce, b0, u, xr);
+        load_x<GROUP, NT, FORM>(a, bounce, b0, u, xr);
         float sum_x[UnitWeights<GROUP>::kGroups][NT];
         group_sums<GROUP, NT>(xr, sum_x);
         f32x4 acc[NT];
@@ -389,7 +401,9 @@ __global__ __launch_bounds__(64 * max_waves(GROUP, NT)) void linear_w4_kernel(Li
         };
         load_slot(0, 0);
         u32x4 xr[2][4][NT];
-        load_x<GROUP, NT>(a, reinterpret_cast<uint8_t*>(part + wave * per_wave), b0, u, xr);
+        uint8_t* const bounce = reinterpret_cast<uint8_t*>(part + wave * per_wave);
+        if (a.x_scales) load_x<GROUP, NT, kRowsE4m3>(a, bounce, b0, u, xr);
+        else load_x<GROUP, NT, kRowsBf16>(a, bounce, b0, u, xr);
         __builtin_amdgcn_sched_barrier(0);  // the other slots' registers are free until x is where it stays
 #pragma unroll
         for (int d = 1; d < D; ++d) load_slot(d, d);
@@ -444,7 +458,14 @@ static int launch_linear_tile(const LinearArgs& a, int n_units, hipStream_t stre
                            stream, a);
         return launch_status();
     };
-    return n_units == waves ? launch(linear_tile_kernel<GROUP, NT, true>) : launch(linear_tile_kernel<GROUP, NT, false>);
+    auto of = [&](auto form) {
+        constexpr int FORM = decltype(form)::value;
+        return n_units == waves ? launch(linear_tile_kernel<GROUP, NT, FORM, true>) : launch(linear_tile_kernel<GROUP, NT, FORM, false>);
+    };
+    if (a.x_scales) return of(std::integral_constant<int, kRowsE4m3>{});
+    if constexpr (NT == 1)
+        if (a.B == 1) return of(std::integral_constant<int, kOneRowBf16>{});
+    return of(std::integral_constant<int, kRowsBf16>{});
 }
 
 template <int GROUP, int NT, int D, int G>
