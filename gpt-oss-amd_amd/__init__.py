@@ -255,6 +255,8 @@ class RouteRule:
     """A routing rule (moe_route_params): scoring "softmax" or "sigmoid", balance_bias fp32 [num_experts] on the device or None."""
 
     def __init__(self, scoring="softmax", balance_bias=None, n_groups=1, groups_per_token=1, group_top=1, renormalize=True, scale=1.0):
+        if scoring not in ("softmax", "sigmoid"):
+            raise ValueError("scoring: expected softmax or sigmoid, got %r" % (scoring,))
         self.balance_bias = balance_bias  # kept alive: the parameters hold its address
         self.params = RouteParams(struct_bytes=ctypes.sizeof(RouteParams),
                                   scoring={"softmax": MOE_ROUTE_SOFTMAX, "sigmoid": MOE_ROUTE_SIGMOID}[scoring], n_groups=n_groups,

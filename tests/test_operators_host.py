@@ -100,6 +100,11 @@ def test_wrappers_refuse_tensors_that_do_not_fit(pkg):
         pkg.linear_int4(x, x.bfloat16(), x, x, 2, 64, 64, 32, x_scales=x)
 
 
+def test_a_rule_is_softmax_or_sigmoid(pkg):
+    with pytest.raises(ValueError, match="scoring: expected softmax or sigmoid, got 'tanh'"):
+        pkg.RouteRule("tanh")
+
+
 def test_oracle_e4m3_and_scales_agree_with_torch():
     import torch
     v = np.concatenate([np.linspace(-448, 448, 4001), np.exp2(np.linspace(-14, 8.8, 999))])
