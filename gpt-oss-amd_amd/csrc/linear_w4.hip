@@ -13,8 +13,8 @@ constexpr int kUnit = 256;  // contraction elements of a wave: two chunks of 128
 
 // Waves of a block at most: what the registers of a wave allow (16: 128, 12: 168, 8: 256).
 constexpr int max_waves(int group, int nt) {
-    if (group == 32) return nt == 2 ? 8 : 12;
-    return group == 64 && nt == 2 ? 12 : 16;
+    if (nt == 1) return 16;
+    return group == 32 ? 8 : group == 64 ? 12 : 16;
 }
 
 // e4m3 values times a power of two, to bf16 (exact: three mantissa bits).
@@ -120,10 +120,20 @@ MOE_DEVICE void load_x(const LinearArgs& a, [[maybe_unused]] uint8_t* bounce, in
     }
 }
 
-// Eight codes 0..15 of a dword (order of int4_repack_kernel) as the bf16 numbers 16..31: the code goes to the mantissa's top four bits.
-MOE_DEVICE u32x4 int4_dword_to_bf16x8(uint32_t w) {
-    constexpr uint32_t kMask = 0x00780078u, kSixteen = 0x41804180u;
-    return u32x4{((w << 3) & kMask) | kSixteen, ((w >> 1) & kMask) | kSixteen, ((w >> 5) & kMask) | kSixteen, ((w >> 9) & kMask) | kSixteen};
+// Codes less their zero point, exact in e4m3: weights without their scale.  Four codes 0..15 in the bytes of `q`, 128 + zero point in every byte of
+// `z`.  A byte u = 128 + z - q with its top bit set is -(z - q) in sign and magnitude as it stands; in the others the magnitude is 128 - u and the
+// sign plus.  Magnitudes up to 15 are e4m3 codes of themselves, in steps of 2^-9.  (The bf16 numbers 16 + code are cheaper to make, with 16 + zero
+// times the sum of x taken off each group's sum.  That loses what cancels between the two, and overflows where the result does not.  So : exact, us, 16
+// rows of 65536 x 2880, scales per 128 24.4 : 25.8, per 64 27.0 : 27.7, per 32 41.6 : 32.1, with room for more waves now.)
+MOE_DEVICE uint32_t int4_less_zero_e4m3(uint32_t q, uint32_t z) {
+    const uint32_t u = z - q;  // no byte borrows from the next
+    const uint32_t positive = ~u & 0x80808080u, one = positive >> 7;
+    return (u ^ (positive - one)) + one;
+}
+// Eight codes of a dword (order of int4_repack_kernel).
+MOE_DEVICE u32x4 int4_dword_to_bf16x8(uint32_t w, uint32_t z) {
+    constexpr uint32_t kCodes = 0x0F0F0F0Fu;
+    return e4m3x8_to_bf16(int4_less_zero_e4m3(w & kCodes, z), int4_less_zero_e4m3((w >> 4) & kCodes, z), 512.f);
 }
 
 }  // namespace
@@ -134,8 +144,8 @@ struct UnitWeights {
     static constexpr int kGroups = GROUP ? kUnit / GROUP : 1;
     u32x4 raw[2];
     uint32_t sw;                      // MXFP4: the scale bytes of four chunks
-    u32x4 sc[GROUP ? kGroups / 2 : 1];  // int4: four rows' scales of two groups
-    u32x2 zp[GROUP ? kGroups / 2 : 1];  // and their zero points
+    u32x4 sc[GROUP ? kGroups / 2 : 1];  // int4: four rows' scales of two groups, those of the lane's results
+    uint32_t zp[2];                     // and a byte zero point ^ 8 for every group of the lane's row of weights
 
     // Unit u of a tile; nothing is read unless `in`, without a branch: the compiler would wait for every load in flight where two paths meet.
     MOE_DEVICE void load(const LinearArgs& a, int tile, int u, bool in) {
@@ -158,15 +168,21 @@ struct UnitWeights {
             const __amdgpu_buffer_rsrc_t z_rsrc =
                 __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.w_zeros) + (size_t)(uint32_t)tile * (scale_bytes / 2), 0,
                                                   in && a.w_zeros ? (int)(scale_bytes / 2) : 0, 0x00020000);
-#pragma unroll
-            for (int i = 0; i < kGroups / 2; ++i)
-                zp[i] = __builtin_amdgcn_raw_buffer_load_b64(z_rsrc, g * kGroups * 4 + i * 8, u * kGroups * 16, 0);
+            const int at = (lane & 15) * kGroups;  // without zero points 0 is read, which stands for 8
+            if constexpr (kGroups == 8) {
+                const u32x2 z = __builtin_amdgcn_raw_buffer_load_b64(z_rsrc, at, u * kGroups * 16, 0);
+                zp[0] = z[0], zp[1] = z[1];
+            } else if constexpr (kGroups == 4) {
+                zp[0] = __builtin_amdgcn_raw_buffer_load_b32(z_rsrc, at, u * kGroups * 16, 0);
+            } else {
+                zp[0] = __builtin_amdgcn_raw_buffer_load_b16(z_rsrc, at, u * kGroups * 16, 0);
+            }
         }
     }
 
     // acc = the unit's products with x, from zero
     template <int NT>
-    MOE_DEVICE void multiply(bool zeros, int u, const u32x4 (&xr)[2][4][NT], const float (&sum_x)[kGroups][NT], f32x4 (&acc)[NT]) const {
+    MOE_DEVICE void multiply(int u, const u32x4 (&xr)[2][4][NT], f32x4 (&acc)[NT]) const {
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t] = zero;
@@ -185,49 +201,28 @@ struct UnitWeights {
                 }
             }
         } else {
-            // sum x (q - z) s = s (sum x (16 + q) - (16 + z) sum x) per group: 16 + q is a bf16 number
             f32x4 p[NT];
+            uint32_t z = 0;
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
-                const u32x4 av = int4_dword_to_bf16x8(raw[n >> 2][n & 3]);
+                const int grp = 32 * n / GROUP;
+                if (32 * n % GROUP == 0) z = __builtin_amdgcn_perm(0u, zp[grp >> 2] ^ 0x88888888u, 0x01010101u * (grp & 3));
+                const u32x4 av = int4_dword_to_bf16x8(raw[n >> 2][n & 3], z);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) p[t] = mfma_16x16x32(av, xr[n >> 2][n & 3][t], 32 * n % GROUP == 0 ? zero : p[t]);
                 if (32 * (n + 1) % GROUP == 0) {
-                    const int grp = 32 * n / GROUP;
-                    const uint32_t zb = zeros ? zp[grp / 2][grp & 1] : 0x18181818u;
                     const uint32_t s01 = sc[grp / 2][2 * (grp & 1)], s23 = sc[grp / 2][2 * (grp & 1) + 1];
                     const float s[4] = {bf16_bits_to_f32(s01 & 0xFFFFu), bf16_bits_to_f32(s01 >> 16), bf16_bits_to_f32(s23 & 0xFFFFu),
                                         bf16_bits_to_f32(s23 >> 16)};
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float z = (float)((zb >> (8 * r)) & 0xFFu);
+                    for (int r = 0; r < 4; ++r)
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) acc[t][r] = fmaf(s[r], fmaf(-z, sum_x[grp][t], p[t][r]), acc[t][r]);
-                    }
-                    if (GROUP < 128) __builtin_amdgcn_sched_barrier(0);  // or all groups' factors are made first, and spilled
+                        for (int t = 0; t < NT; ++t) acc[t][r] = fmaf(s[r], p[t][r], acc[t][r]);
                 }
             }
         }
     }
 };
-
-// Sums of x over the groups of a unit, by a product with ones: every row of the result is the sums of its columns.
-template <int GROUP, int NT>
-MOE_DEVICE void group_sums(const u32x4 (&xr)[2][4][NT], float (&sum_x)[UnitWeights<GROUP>::kGroups][NT]) {
-    if constexpr (GROUP != 0) {
-        const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            f32x4 s;
-#pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                if (32 * n % GROUP == 0) s = f32x4{0.f, 0.f, 0.f, 0.f};
-                s = mfma_16x16x32(ones, xr[n >> 2][n & 3][t], s);
-                if (32 * (n + 1) % GROUP == 0) sum_x[32 * n / GROUP][t] = s[0];
-            }
-        }
-    }
-}
 
 // Weight row of row r of a tile.
 template <int GROUP>
@@ -276,10 +271,8 @@ __global__ __launch_bounds__(64 * max_waves(GROUP, NT)) void linear_tile_kernel(
         w.load(a, tile, u, true);
         u32x4 xr[2][4][NT];
         load_x<GROUP, NT, FORM>(a, bounce, b0, u, xr);
-        float sum_x[UnitWeights<GROUP>::kGroups][NT];
-        group_sums<GROUP, NT>(xr, sum_x);
         f32x4 acc[NT];
-        w.template multiply<NT>(a.w_zeros != nullptr, u, xr, sum_x, acc);
+        w.template multiply<NT>(u, xr, acc);
 #pragma unroll
         for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(part + (u * NT + t) * 256 + lane * 4) = acc[t];
         if constexpr (ONE) break;
@@ -407,13 +400,11 @@ __global__ __launch_bounds__(64 * max_waves(GROUP, NT)) void linear_w4_kernel(Li
         __builtin_amdgcn_sched_barrier(0);  // the other slots' registers are free until x is where it stays
 #pragma unroll
         for (int d = 1; d < D; ++d) load_slot(d, d);
-        float sum_x[UnitWeights<GROUP>::kGroups][NT];
-        group_sums<GROUP, NT>(xr, sum_x);
         // partial tile of set j, in slot S of the ring, the m-th of its step
         auto tile_part = [&](auto slot_tag, int m, int j) {
             constexpr int S = decltype(slot_tag)::value;
             f32x4 acc[NT];
-            w[S].template multiply<NT>(a.w_zeros != nullptr, u, xr, sum_x, acc);
+            w[S].template multiply<NT>(u, xr, acc);
             __builtin_amdgcn_sched_barrier(0);
             load_slot(S, j + D);  // the slot is free
             __builtin_amdgcn_sched_barrier(0);
@@ -503,9 +494,9 @@ static int launch_linear_rows(const LinearArgs& a, int n_cus, hipStream_t stream
     const int at_once = NT == 1 ? std::clamp(24 / n_units, 1, 3) : 1;
     if (tiles <= (long long)n_cus * at_once && linear_tile_lds(GROUP, NT, n_units) <= kLdsMost) return launch_linear_tile<GROUP, NT>(a, n_units, stream);
     // With up to three tiles to a block the longer ring and the wider steps of the second form cost more code than they hide: us, first : second
-    // form, 64 rows of 5760 x 2880 int4 10.6 : 11.1, 1 row of 16384 x 4096 MXFP4 11.7 : 10.1, 16 rows of 131072 x 2880 42.7 : 38.6.  More than 128 int4 scales to a tile's unit, those per 64 with 32 rows and those per 32, do not fit a ring of two.
-    if (tiles <= 3LL * n_cus || GROUP == 32 || (GROUP == 64 && NT == 2)) return launch_linear_of<GROUP, NT, 1, 2>(a, n_cus, stream);
-    if constexpr (!(GROUP == 32 || (GROUP == 64 && NT == 2))) return launch_linear_of<GROUP, NT, 2, 4 / NT>(a, n_cus, stream);
+    // form, 64 rows of 5760 x 2880 int4 10.6 : 11.1, 1 row of 16384 x 4096 MXFP4 11.7 : 10.1, 16 rows of 131072 x 2880 42.7 : 38.6.  int4 scales per 32 need the registers of a ring of two for more waves (65536 x 2880, 16 rows, 16 waves : 12 with the ring, 32.3 : 37.4).
+    if (tiles <= 3LL * n_cus || GROUP == 32) return launch_linear_of<GROUP, NT, 1, 2>(a, n_cus, stream);
+    if constexpr (GROUP != 32) return launch_linear_of<GROUP, NT, 2, 4 / NT>(a, n_cus, stream);
     return MOE_ERR_LIMIT;
 }
 
@@ -527,9 +518,10 @@ int launch_linear_w4(const LinearArgs& args, int group, int n_cus, hipStream_t s
 
 // ---- int4 codes ------------------------------------------------------------------------------------
 // Tiles of 16 weight rows, a tile's contraction in chunks of 128 elements (the last one filled up with zeros), lane 16 g + r of a chunk's
-// 1 KiB: dword j holds elements 32 j + 8 g .. + 8 of row r, the element pair 2p, 2p + 1 at bits 4p and 16 + 4p, so that a shift and a mask leave a
-// pair at the same place of a dword's two halves.  Scales bf16, zero points as the byte 16 + z, both [tile][unit of 256][4 lane groups]
-// [groups of the unit][4 rows]: a lane reads those of the four rows it gets from the matrix instruction in one piece; 0 past the last row and group.
+// 1 KiB: dword j holds elements 32 j + 8 g .. + 8 of row r, the first four in the low halves of its bytes, the others in the high ones.
+// Scales bf16 [tile][unit of 256][4 lane groups][groups of the unit][4 rows]: a lane reads those of the four rows it gets from the matrix instruction
+// in one piece.  Zero points as the byte z ^ 8 [tile][unit][16 rows][groups of the unit]: a lane reads those of the row it unpacks.  0 past the last
+// row and group.
 void int4_tiled_bytes(int rows, int K, int group, size_t* codes, size_t* scales, size_t* zeros) {
     const size_t tiles = (size_t)ceil_div(rows, 16), groups = (size_t)ceil_div(K, kUnit) * (kUnit / group);
     if (codes) *codes = tiles * (size_t)ceil_div(K, 128) * 1024;
@@ -552,7 +544,7 @@ __global__ __launch_bounds__(256) void int4_repack_kernel(const uint32_t* __rest
         if (row < rows && k < K) {
             const uint32_t w = codes[(size_t)row * (K / 8) + k / 8];
 #pragma unroll
-            for (int p = 0; p < 4; ++p) v[j] |= ((w >> (8 * p)) & 0xFu) << (4 * p) | ((w >> (8 * p + 4)) & 0xFu) << (16 + 4 * p);
+            for (int e = 0; e < 8; ++e) v[j] |= ((w >> (4 * e)) & 0xFu) << (8 * (e & 3) + 4 * (e >> 2));
         }
     }
     out[i] = v;
@@ -566,13 +558,16 @@ __global__ __launch_bounds__(256) void int4_scales_repack_kernel(const uint16_t*
     const int per_unit = kUnit / group, n_units = ceil_div(K, kUnit), n_groups = ceil_div(K, group);
     const long long unit = i / (16 * per_unit);  // over all tiles
     const int in_unit = (int)(i - unit * (16 * per_unit));
-    const int g = in_unit / (4 * per_unit), grp = in_unit / 4 % per_unit;
-    const long long row = unit / n_units * 16 + 4 * g + (in_unit & 3);
-    const long long at = unit % n_units * per_unit + grp;
-    const bool in = row < rows && at < n_groups;
-    const size_t src = in ? (size_t)row * n_groups + (size_t)at : 0;
-    out_scales[i] = in ? scales[src] : 0;
-    if (zeros) out_zeros[i] = in ? (uint8_t)(16 + (zeros[src] & 15)) : 0;
+    const long long row0 = unit / n_units * 16, group0 = unit % n_units * per_unit;
+    auto source = [&](int row, int grp) {  // -1: past the last row or group
+        return row0 + row < rows && group0 + grp < n_groups ? (row0 + row) * n_groups + group0 + grp : -1ll;
+    };
+    const long long s = source(in_unit / (4 * per_unit) * 4 + (in_unit & 3), in_unit / 4 % per_unit);
+    out_scales[i] = s >= 0 ? scales[s] : 0;
+    if (zeros) {
+        const long long z = source(in_unit / per_unit, in_unit % per_unit);
+        out_zeros[i] = z >= 0 ? (uint8_t)((zeros[z] & 15) ^ 8) : 0;
+    }
 }
 
 int launch_int4_repack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int rows, int K, int group, uint8_t* tiled_codes,

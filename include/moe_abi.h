@@ -305,8 +305,8 @@ MOE_API int moe_add_rmsnorm(float* x_out, const float* x, const float* delta, co
  * moe_linear_mxfp4: tiled_blocks / tiled_scales of moe_mxfp4_repack(E = 1, rows = N, K); N % 64 == 0.
  *
  * moe_linear_int4: W[n, k] = (code - zero) * scale, codes 0..15, one bf16 scale and one zero point 0..15 for every `group` (32, 64 or 128) values of a
- * row, the last group of which may be shorter; any N.  tiled_* come from moe_int4_repack; tiled_zeros NULL: zero points of 8.  A row of
- * x with an infinity or a NaN may give NaN where exact arithmetic gives an infinity. */
+ * row, the last group of which may be shorter; any N.  tiled_* come from moe_int4_repack; tiled_zeros NULL: zero points of 8.  code - zero is
+ * taken exactly and the scale put to the sum of up to 128 products x (code - zero) of a group: past 2^128 that sum is an infinity, whatever the scale. */
 MOE_API int moe_linear_mxfp4(float* y, const void* x, const uint8_t* x_scales, const uint8_t* tiled_blocks, const uint8_t* tiled_scales,
                              const moe_bf16_t* bias, int B, int K, int N, moe_stream_t stream);
 MOE_API int moe_linear_int4(float* y, const void* x, const uint8_t* x_scales, const uint8_t* tiled_codes, const moe_bf16_t* tiled_scales,
