@@ -21,53 +21,51 @@ struct RouteCut {
 };
 
 // ---- scores ---------------------------------------------------------------------------------------
-// 2^t for |t| <= 200: the Taylor series of 2^f, f = t - rint(t), to the 11th power (relative error 2^-47).
-MOE_DEVICE double exp2_series(double t) {
-    const double n = __builtin_rint(t), f = t - n;
-    constexpr double kLn2 = 0.693147180559945309417;
-    // ln2^i / i!
-    constexpr double c2 = kLn2 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4, c5 = c4 * kLn2 / 5, c6 = c5 * kLn2 / 6, c7 = c6 * kLn2 / 7,
-                     c8 = c7 * kLn2 / 8, c9 = c8 * kLn2 / 9, c10 = c9 * kLn2 / 10, c11 = c10 * kLn2 / 11;
-    double p = c11;
-    p = fma(p, f, c10);
-    p = fma(p, f, c9);
-    p = fma(p, f, c8);
-    p = fma(p, f, c7);
-    p = fma(p, f, c6);
-    p = fma(p, f, c5);
-    p = fma(p, f, c4);
-    p = fma(p, f, c3);
-    p = fma(p, f, c2);
-    p = fma(p, f, kLn2);
+// exp(x) for |x| <= 139, to 2^-52: 2^f from the polynomial that meets it at the twelve Chebyshev nodes of -1/2 .. 1/2 (2^-57; as many terms of the
+// Taylor series give 2^-47), f = x log2(e) less the whole number next to it, log2(e) in two parts.
+MOE_DEVICE double exp_series(double x) {
+    const double n = __builtin_rint(x * 0x1.71547652b82fep+0);
+    const double f = fma(x, 2.0355273740931033e-17, fma(x, 0x1.71547652b82fep+0, -n));
+    double p = 0x1.e9ec1fcb69a7fp-32;
+    p = fma(p, f, 0x1.e6228acd1c6e5p-28);
+    p = fma(p, f, 0x1.b524ebd13a55fp-24);
+    p = fma(p, f, 0x1.62bfc2c86d700p-20);
+    p = fma(p, f, 0x1.ffcbfc6da6ed1p-17);
+    p = fma(p, f, 0x1.430913112c61bp-13);
+    p = fma(p, f, 0x1.5d87fe78a3f9cp-10);
+    p = fma(p, f, 0x1.3b2ab6fb9f1a5p-7);
+    p = fma(p, f, 0x1.c6b08d704a0c6p-5);
+    p = fma(p, f, 0x1.ebfbdff82c5aep-3);
+    p = fma(p, f, 0x1.62e42fefa39efp-1);
     p = fma(p, f, 1.0);
     return __builtin_ldexp(p, (int)n);
 }
-constexpr double kLog2e = 1.44269504088896340736;
 
-// 1 / d for 1 <= d < 2^250: the hardware's estimate (2^-24) and a step of Newton's iteration (2^-48).
+// 1 / d for 1 <= d < 2^250: the hardware's estimate (2^-24) and a step of third order.
 MOE_DEVICE double reciprocal(double d) {
-    const double r = __builtin_amdgcn_rcp(d);
-    return fma(fma(-d, r, 1.0), r, r);
+    const double r = __builtin_amdgcn_rcp(d), e = fma(-d, r, 1.0);
+    return fma(r, fma(e, e, e), r);
 }
 
-// 1 / (1 + exp(-l)), rounded to fp32 once.  Past 130 either way the result is 0 or 1 in fp32.
+// 1 / (1 + exp(-l)) to 2^-51, rounded to fp32 once.  Past 130 either way the result is 0 or 1 in fp32.
 MOE_DEVICE float sigmoid_score(float l) {
     const float near = fminf(fmaxf(l, -130.f), 130.f);
-    const float s = (float)reciprocal(1.0 + exp2_series((double)near * -kLog2e));
+    const float s = (float)reciprocal(1.0 + exp_series(-(double)near));
     return l == l ? s : l;
 }
 
-// exp(l - mx), from 2^-200 on: what is less is 0 in fp32 whatever it is divided by.
-MOE_DEVICE double softmax_term(float l, double mx) { return exp2_series(fmax(((double)l - mx) * kLog2e, -200.0)); }
+// exp(l - mx), from exp(-138) on: what is less is 0 in fp32 whatever it is divided by.  (An infinite mx leaves no number above that.)
+MOE_DEVICE double softmax_term(float l, double mx) { return exp_series(fmax((double)l - mx, -138.0)); }
 
-// What the terms of a row with largest logit mx (a NaN if it holds one) are multiplied by: 0 where all logits are -infinity.
-MOE_DEVICE double softmax_scale(float mx, double sum) {
+// A row's sum of terms in whole numbers of 2^-52 (terms are 0 .. 1), so that it does not depend on how the row lies over lanes, and a token
+// gets the same bits in a batch of any size: the bits of 1 + term rise by one for each.
+MOE_DEVICE uint64_t term_units(double e) { return __builtin_bit_cast(uint64_t, e + 1.0) - __builtin_bit_cast(uint64_t, 1.0); }
+
+// What the terms of a row with largest logit mx (+infinity if it holds a NaN) are multiplied by: 0 where all logits are -infinity.
+MOE_DEVICE double softmax_scale(float mx, uint64_t units) {
     if (mx == -INFINITY) return 0.0;
-    return mx < INFINITY ? reciprocal(sum) : (double)NAN;
+    return mx < INFINITY ? reciprocal((double)units * 0x1p-52) : (double)NAN;
 }
-
-// The largest logit as the terms want it: finite.
-MOE_DEVICE double softmax_base(float mx) { return fabsf(mx) < INFINITY ? (double)mx : 0.0; }
 
 // ---- values with their place ------------------------------------------------------------------------
 // A choice value and its place as one double, which v_max_f64 ranks by value and then by lower place: an fp32 value leaves 29 bits of the
@@ -136,6 +134,14 @@ MOE_DEVICE double token_reduce(double v, Op op) {
     return v;
 }
 
+template <int LPT>
+MOE_DEVICE uint64_t token_sum(uint64_t v) {
+    const double sum = token_reduce<LPT>(__builtin_bit_cast(double, v), [](double a, double b) {
+        return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, a) + __builtin_bit_cast(uint64_t, b));
+    });
+    return __builtin_bit_cast(uint64_t, sum);
+}
+
 // (a, b) in descending order
 MOE_DEVICE void descending(double& a, double& b) {
     const double hi = larger(a, b), lo = smaller(a, b);
@@ -191,12 +197,13 @@ MOE_DEVICE void top_descending(double (&d)[V]) {
 
 // LPT lanes to a token (64 / LPT tokens to a wave), up to V experts to a lane, a group of experts in whole lanes.
 //   s = 1 / (1 + exp(-l))  or  exp(l - max) / sum, in fp64, rounded to fp32 once: scores that differ in their last place decide between
-//   experts, and a rule stated on rounded scores has one answer whatever computes it
+//   experts, and a rule stated on rounded scores has one answer whatever computes it to fp64's accuracy (but for one score in some 2^26 that lies that
+//   near the middle of two fp32 numbers)
 //   c = s + bias; group value = sum of the group_top largest c of its experts; the groups_per_token largest groups stay
 //   K largest c of the groups that stay (equal ones: the lower index); weight = s / (sum over the chosen) * scale
-// Bound by its instructions: some 26 in 64 bits for every score, 300 a token (of 256 experts, 8 of them chosen) for the selection.  A lane sorts its
+// Bound by its instructions: some 28 in 64 bits for every score, 300 a token (of 256 experts, 8 of them chosen) for the selection.  A lane sorts its
 // values once; a round of the selection is then a maximum over the first of every lane's, and the lane that had it moves up its next.
-// 16384 tokens of 256 experts: a wave a token, keys searched in every round, the library's exponential 24.6 us, so 12.0 (2.4 of them are
+// 16384 tokens of 256 experts: a wave a token, keys searched in every round, the library's exponential 24.6 us, so 12.4 (2.4 of them are
 // an empty launch's); 2.6 would be the logits at the rate of a long read.
 template <int LPT, int V, int KMAX>
 __global__ __launch_bounds__(256) void route_kernel(const float* __restrict__ logits, float* __restrict__ topk_v, int* __restrict__ topk_i, int T,
@@ -245,14 +252,14 @@ __global__ __launch_bounds__(256) void route_kernel(const float* __restrict__ lo
             nan |= s[v] != s[v];
         }
         const float mx = (float)token_reduce<LPT>(nan ? (double)INFINITY : most, larger);
-        const double base = softmax_base(mx);
-        double e[V], sum = 0.0;
+        double e[V];
+        uint64_t units = 0;  // places without an expert have terms that round to none
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            e[v] = softmax_term(s[v], base);
-            sum += v < n ? e[v] : 0.0;
+            e[v] = softmax_term(s[v], (double)mx);
+            units += term_units(e[v]);
         }
-        const double scale = softmax_scale(mx, token_reduce<LPT>(sum, [](double a, double b) { return a + b; }));
+        const double scale = softmax_scale(mx, token_sum<LPT>(units));
 #pragma unroll
         for (int v = 0; v < V; ++v) s[v] = (float)(e[v] * scale);
     } else {
@@ -372,14 +379,14 @@ __global__ __launch_bounds__(256) void route_any_kernel(const float* __restrict_
         MOE_DPP_STEPS(MOE_STEP)
 #undef MOE_STEP
         const float mx = rank_key_value(__builtin_amdgcn_readlane(best, 63));
-        const double base = softmax_base(mx);
-        double e[C], sum = 0.0;
+        double e[C];
+        uint64_t units = 0;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            e[c] = softmax_term(l[c], base);
-            sum += lane + 64 * c < E ? e[c] : 0.0;
+            e[c] = softmax_term(l[c], (double)mx);
+            units += term_units(e[c]);
         }
-        const double scale = softmax_scale(mx, wave_sum(sum));
+        const double scale = softmax_scale(mx, token_sum<64>(units));
 #pragma unroll
         for (int c = 0; c < C; ++c) s[c] = (float)(e[c] * scale);
     } else {

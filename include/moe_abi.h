@@ -123,8 +123,9 @@ MOE_API int moe_softmax(float* x, int batch_size, int size, moe_stream_t stream)
 
 /* Routing by score: router logits -> topk_values / topk_indices [batch_size, experts_per_token], for models whose rule is not
  * "softmax over the largest logits" (moe_topk + moe_softmax).  No counterpart in the reference.  Per token, with l its logits:
- *   score[e]  = 1 / (1 + exp(-l[e]))  or  exp(l[e] - max l) / sum exp(l - max l), computed in fp64 and rounded to fp32; a logit of
- *               -infinity scores 0 (so does a token's every expert if all its logits are)
+ *   score[e]  = 1 / (1 + exp(-l[e]))  or  exp(l[e] - max l) / sum exp(l - max l), computed in fp64 (to about 2^-51; the sum's terms to 2^-53
+ *               of the largest) and rounded to fp32: the nearest, but for a score that near the middle of two.  The same bits in a batch of
+ *               any size.  A logit of -infinity scores 0 (so does a token's every expert if all its logits are)
  *   choice[e] = score[e] + balance_bias[e]  (fp32; score[e] without a bias)
  *   groups    : experts form n_groups runs of num_experts / n_groups; a group's value is the sum (fp32) of its group_top largest choices
  *               (group_top 1 or 2; a group of one expert has one); the groups_per_token groups of largest value stay, equal ones: the lower
