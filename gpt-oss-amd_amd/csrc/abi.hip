@@ -141,9 +141,9 @@ struct BlockWorkspace {
     int* fused_ctr;        // counters of the one-launch expert kernel (experts_fused.hip)
     uint16_t* h_by_slot;   // [A, I] bf16 SwiGLU outputs
     float* y_by_slot;      // [A, H] fp32 down-projection rows
-    float* logits;         // [T,E] for a routing rule
+    float* logits;         // [T,E] for a routing rule: where the experts' rows come later, unless these are too short for it
     int max_tiles;
-    size_t bytes;
+    size_t bytes, rule_bytes;  // without, and with such logits
 
     BlockWorkspace(void* base, int T, int H, int I, int E, int K) {
         const size_t A = (size_t)T * K;
@@ -167,10 +167,12 @@ struct BlockWorkspace {
         tile_rows = static_cast<int*>(take((size_t)2 * max_tiles * 4));
         n_tiles = static_cast<int*>(take(4));
         fused_ctr = static_cast<int*>(take((size_t)expert_fused_ctr_words(E) * 4));
+        const size_t rows = off, logits_bytes = (size_t)T * E * 4;
         h_by_slot = static_cast<uint16_t*>(take(A * I * 2));
         y_by_slot = static_cast<float*>(take(A * H * 4));
-        logits = static_cast<float*>(take((size_t)T * E * 4));
         bytes = off;
+        logits = logits_bytes <= bytes - rows ? reinterpret_cast<float*>(h_by_slot) : static_cast<float*>(take(logits_bytes));
+        rule_bytes = off;
     }
 };
 
@@ -656,7 +658,7 @@ size_t moe_block_workspace_bytes(int n_tokens, int hidden_dim, int intermediate_
     // and 64 tokens, so a smaller batch may need more.
     size_t most = 0;
     for (int t = n_tokens; t > 0; t = (t - 1) / 16 * 16)
-        most = std::max(most, BlockWorkspace(nullptr, t, hidden_dim, intermediate_dim, n_experts, experts_per_token).bytes);
+        most = std::max(most, BlockWorkspace(nullptr, t, hidden_dim, intermediate_dim, n_experts, experts_per_token).rule_bytes);
     return most;
 }
 
@@ -854,7 +856,7 @@ static int block_forward_impl(const moe_block_params* caller, moe_stream_t strea
         return MOE_ERR_ALIGN;
     if (!p->workspace || ((uintptr_t)p->workspace & (kAlign - 1))) return MOE_ERR_WORKSPACE;
     BlockWorkspace ws(p->workspace, T, H, I, E, K);
-    if (p->workspace_bytes < ws.bytes) return MOE_ERR_WORKSPACE;
+    if (p->workspace_bytes < (p->route && !p->router_score ? ws.rule_bytes : ws.bytes)) return MOE_ERR_WORKSPACE;
     hipStream_t stream = as_stream(stream_);
     int stage = 0;
     auto mark = [&]() -> int {

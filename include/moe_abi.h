@@ -394,7 +394,8 @@ typedef struct moe_block_params {
     const moe_bf16_t* next_norm_weight; /* [H] */
     float* next_norm_out;               /* [B,H] */
     /* Optional: the routing rule (host memory, read during the call) in place of top-k and softmax over the chosen, applied to the router's
-     * logits (exact ones, as moe_gemm_router).  topk_i / topk_v are then what moe_route gives.  A caller built against the struct
+     * logits (exact ones, as moe_gemm_router; kept in the workspace if router_score is NULL, which takes no more of it unless
+     * 4 n_experts > experts_per_token (2 intermediate_dim + 4 hidden_dim)).  topk_i / topk_v are then what moe_route gives.  A caller built against the struct
      * without this member gets the behaviour of NULL. */
     const moe_route_params* route;
 } moe_block_params;

@@ -1,0 +1,15 @@
+"""A routing rule takes no room in the block's workspace that its experts' rows do not have."""
+import pytest
+
+
+@pytest.mark.parametrize("shape,nbytes", [((1, 2880, 2880, 32, 4), 82176), ((256, 2880, 2880, 32, 4), 20232448), ((4096, 2880, 2880, 32, 4), 318632448),
+                                          ((4096, 2880, 2880, 128, 4), 322563584), ((16384, 2880, 2880, 128, 8), 2411650816),
+                                          ((300, 64, 64, 16, 2), 316416)])
+def test_sizes_are_those_of_the_block_without_rules(pkg, shape, nbytes):
+    assert pkg.block_workspace_bytes(*shape) == nbytes
+
+
+def test_logits_longer_than_the_rows_have_room_of_their_own(pkg):
+    """64 experts' rows of one bf16 and one fp32 row a token against 128 and 1024 logits: T * E * 4 bytes more."""
+    assert pkg.block_workspace_bytes(8, 64, 64, 128, 1) == 18688 + 8 * 128 * 4
+    assert pkg.block_workspace_bytes(500, 64, 64, 1024, 1) == 4392448 + 500 * 1024 * 4
