@@ -574,11 +574,10 @@ int moe_linear_int4(float* y, const void* x, const uint8_t* x_scales, const uint
                             device_cu_count(), as_stream(stream));
 }
 
-// the repack's grids count 256 lanes, and scales, to a block
 static int check_int4(int rows, int K, int group) {
     if (rows <= 0 || K <= 0 || K % 32 != 0) return MOE_ERR_SHAPE;
     if (group != 32 && group != 64 && group != 128) return MOE_ERR_FORMAT;
-    if ((long long)ceil_div(rows, 16) * ceil_div(K, 32) * 16 > 0x7FFFFFFFll * 256) return MOE_ERR_LIMIT;
+    if (rows > kMostRows || K > kMostRows) return MOE_ERR_LIMIT;  // counted up to whole tiles in 32 bits
     return MOE_OK;
 }
 

@@ -1,4 +1,5 @@
 // Residual add, RMSNorm and its result in the type the next product reads: fp32, bf16, or e4m3 with scales.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -218,6 +219,21 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void add_rmsnorm_ker
 // (142 MB) 27.4 : 28.3 and 1000 in bf16 9.0 : 9.5.
 static bool past_cache(const AddNormArgs& a, int batch) { return (long long)batch * a.size * (a.delta ? 12 : 8) > (256ll << 20); }
 
+// The arguments for the rows from `row` on.
+static AddNormArgs rows_from(AddNormArgs a, long long row) {
+    const long long at = row * a.size;
+    a.x_out += at;
+    a.x += at;
+    if (a.delta) a.delta += at;
+    if (a.o) a.o += at;
+    if (a.o_bf16) a.o_bf16 += at;
+    if (a.q) {
+        a.q += at;
+        a.q_scales += row * (a.q_group == MOE_Q_GROUP_MX ? a.size / 32 : a.q_group == MOE_Q_GROUP_128 ? 4 * ((a.size - 1) / 128 + 1) : 4);
+    }
+    return a;
+}
+
 // Threads to a row by its length: 64 up to 1024 values (16384 rows of 64 9.3 us, with 256 18.1), 256 up to 4096, 512 up to 8192 (64 rows of 8192 5.2 us,
 // with 256 and no values in registers 8.3; 5000 rows 85 : 112), 1024 past that.
 int launch_add_rmsnorm(const AddNormArgs& a, int batch, hipStream_t stream) {
@@ -226,8 +242,14 @@ int launch_add_rmsnorm(const AddNormArgs& a, int batch, hipStream_t stream) {
         constexpr bool NT = decltype(nt)::value;
         auto launch = [&](auto kernel, int threads) {
             const int rows = threads < 256 ? 256 / threads : 1;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(batch, rows)), dim3(threads * rows), 0, stream, a, batch);
-            return launch_status();
+            const long long most = kMostThreads / threads;
+            for (long long row = 0; row < batch; row += most) {
+                const int n = (int)std::min(batch - row, most);
+                hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(n, rows)), dim3(threads * rows), 0, stream, rows_from(a, row), n);
+                const int rc = launch_status();
+                if (rc) return rc;
+            }
+            return (int)MOE_OK;
         };
         if (a.size <= 256) return launch(add_rmsnorm_kernel<64, 1, Q, NT>, 64);
         if (a.size <= 512) return launch(add_rmsnorm_kernel<64, 2, Q, NT>, 64);

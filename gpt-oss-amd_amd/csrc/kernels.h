@@ -41,6 +41,8 @@ int launch_router_two_pass(const float* x, const uint16_t* w, const uint16_t* bi
                            hipStream_t stream, hipEvent_t between, float* approx_out = nullptr,
                            float* delta_out = nullptr, int* n_cand_out = nullptr);
 
+constexpr long long kMostThreads = 1ll << 31;  // of a launch in one dimension; the runtime refuses 2^32
+
 // ---- route.hip --------------------------------------------------------------------------------
 struct RouteRule {  // moe_route_params
     const float* bias;

@@ -531,52 +531,53 @@ void int4_tiled_bytes(int rows, int K, int group, size_t* codes, size_t* scales,
 
 __global__ __launch_bounds__(256) void int4_repack_kernel(const uint32_t* __restrict__ codes, u32x4* __restrict__ out, int rows, int K,
                                                           long long n_lanes) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n_lanes) return;
     const int n_chunks = ceil_div(K, 128);
-    const long long chunk = i >> 6;
-    const int lane = (int)(i & 63), c = (int)(chunk % n_chunks);
-    const long long row = chunk / n_chunks * 16 + (lane & 15);
-    u32x4 v = {0u, 0u, 0u, 0u};
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n_lanes; i += (long long)gridDim.x * 256) {
+        const long long chunk = i >> 6;
+        const int lane = (int)(i & 63), c = (int)(chunk % n_chunks);
+        const long long row = chunk / n_chunks * 16 + (lane & 15);
+        u32x4 v = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int k = 128 * c + 32 * j + 8 * (lane >> 4);
-        if (row < rows && k < K) {
-            const uint32_t w = codes[(size_t)row * (K / 8) + k / 8];
+        for (int j = 0; j < 4; ++j) {
+            const int k = 128 * c + 32 * j + 8 * (lane >> 4);
+            if (row < rows && k < K) {
+                const uint32_t w = codes[(size_t)row * (K / 8) + k / 8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[j] |= ((w >> (4 * e)) & 0xFu) << (8 * (e & 3) + 4 * (e >> 2));
+                for (int e = 0; e < 8; ++e) v[j] |= ((w >> (4 * e)) & 0xFu) << (8 * (e & 3) + 4 * (e >> 2));
+            }
         }
+        out[i] = v;
     }
-    out[i] = v;
 }
 
 __global__ __launch_bounds__(256) void int4_scales_repack_kernel(const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros,
                                                                  uint16_t* __restrict__ out_scales, uint8_t* __restrict__ out_zeros, int rows,
                                                                  int K, int group, long long n) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
     const int per_unit = kUnit / group, n_units = ceil_div(K, kUnit), n_groups = ceil_div(K, group);
-    const long long unit = i / (16 * per_unit);  // over all tiles
-    const int in_unit = (int)(i - unit * (16 * per_unit));
-    const long long row0 = unit / n_units * 16, group0 = unit % n_units * per_unit;
-    auto source = [&](int row, int grp) {  // -1: past the last row or group
-        return row0 + row < rows && group0 + grp < n_groups ? (row0 + row) * n_groups + group0 + grp : -1ll;
-    };
-    const long long s = source(in_unit / (4 * per_unit) * 4 + (in_unit & 3), in_unit / 4 % per_unit);
-    out_scales[i] = s >= 0 ? scales[s] : 0;
-    if (zeros) {
-        const long long z = source(in_unit / per_unit, in_unit % per_unit);
-        out_zeros[i] = z >= 0 ? (uint8_t)((zeros[z] & 15) ^ 8) : 0;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const long long unit = i / (16 * per_unit);  // over all tiles
+        const int in_unit = (int)(i - unit * (16 * per_unit));
+        const long long row0 = unit / n_units * 16, group0 = unit % n_units * per_unit;
+        auto source = [&](int row, int grp) {  // -1: past the last row or group
+            return row0 + row < rows && group0 + grp < n_groups ? (row0 + row) * n_groups + group0 + grp : -1ll;
+        };
+        const long long s = source(in_unit / (4 * per_unit) * 4 + (in_unit & 3), in_unit / 4 % per_unit);
+        out_scales[i] = s >= 0 ? scales[s] : 0;
+        if (zeros) {
+            const long long z = source(in_unit / per_unit, in_unit % per_unit);
+            out_zeros[i] = z >= 0 ? (uint8_t)((zeros[z] & 15) ^ 8) : 0;
+        }
     }
 }
 
 int launch_int4_repack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int rows, int K, int group, uint8_t* tiled_codes,
                        uint16_t* tiled_scales, uint8_t* tiled_zeros, hipStream_t stream) {
     const long long lanes = (long long)ceil_div(rows, 16) * ceil_div(K, 128) * 64;
-    hipLaunchKernelGGL(int4_repack_kernel, dim3((unsigned)ceil_div(lanes, 256ll)), dim3(256), 0, stream,
+    const auto blocks = [](long long items) { return dim3((unsigned)std::min(ceil_div(items, 256ll), kMostThreads / 256)); };
+    hipLaunchKernelGGL(int4_repack_kernel, blocks(lanes), dim3(256), 0, stream,
                        reinterpret_cast<const uint32_t*>(codes), reinterpret_cast<u32x4*>(tiled_codes), rows, K, lanes);
     const long long n = (long long)ceil_div(rows, 16) * ceil_div(K, kUnit) * (kUnit / group) * 16;
-    hipLaunchKernelGGL(int4_scales_repack_kernel, dim3((unsigned)ceil_div(n, 256ll)), dim3(256), 0, stream, scales, zeros, tiled_scales,
+    hipLaunchKernelGGL(int4_scales_repack_kernel, blocks(n), dim3(256), 0, stream, scales, zeros, tiled_scales,
                        tiled_zeros, rows, K, group, n);
     return launch_status();
 }

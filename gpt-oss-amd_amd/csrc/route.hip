@@ -1,6 +1,7 @@
 // Routing by score: router logits -> the experts of every token and their weights, for rules other than "softmax over the largest
 // logits" (router.hip): softmax or sigmoid scores, a bias that takes part in the choice only, groups of experts, weights
 // renormalised over the chosen and scaled.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -468,15 +469,16 @@ __global__ __launch_bounds__(256) void route_any_kernel(const float* __restrict_
     }
 }
 
-int launch_route(const float* logits, float* topk_v, int* topk_i, int T, int E, int K, const RouteRule& rule, int n_cus,
-                 hipStream_t stream) {
+// Tokens T of a batch of `total`, which is what the lanes of a token go by.
+static int launch_route_part(const float* logits, float* topk_v, int* topk_i, int T, int total, int E, int K, const RouteRule& rule, int n_cus,
+                             hipStream_t stream) {
     const int G = rule.n_groups, size = E / G;
     // Lanes of a token: the fewer, the less a token's exchanges between lanes cost, as long as there are three waves to a compute unit.  us at 16 :
     // 32 : 64 lanes, 256 experts in 8 groups, K = 8, 1 token 5.0 : 4.3 : 4.0, 512 tokens 5.6 : 4.6 : 4.4, 2000 tokens 5.6 : 4.8 : 5.1, 4096 tokens 6.2 :
     // 6.3 : 7.3, 16384 tokens 12.1 : 13.9 : 18.7; 32 experts, 4096 tokens 3.0 : 3.1 : 3.8.  (8 lanes of 32 experts 12.7; blocks that go through
     // several batches of tokens, the next one's logits in flight, 14.5.)
     int lanes = 16;
-    while (lanes < 64 && (long long)T * lanes < 192LL * n_cus) lanes *= 2;
+    while (lanes < 64 && (long long)total * lanes < 192LL * n_cus) lanes *= 2;
     for (int lpt = lanes; lpt <= 64; lpt *= 2) {
         RouteCut cut;
         cut.log_group_lanes = 0;
@@ -507,6 +509,16 @@ int launch_route(const float* logits, float* topk_v, int* topk_i, int T, int E, 
     // over 512 experts in groups that leave lanes idle, as 3 of 320: 16 experts a lane do not do
     hipLaunchKernelGGL(route_any_kernel<16>, dim3((unsigned)ceil_div(T, 4)), dim3(256), 0, stream, logits, topk_v, topk_i, T, E, K, rule);
     return launch_status();
+}
+
+int launch_route(const float* logits, float* topk_v, int* topk_i, int T, int E, int K, const RouteRule& rule, int n_cus,
+                 hipStream_t stream) {
+    constexpr long long kTokens = kMostThreads / 64;  // a multiple of four rows, which keeps the logits' alignment
+    for (long long t = 0; t < T; t += kTokens) {
+        const int rc = launch_route_part(logits + t * E, topk_v + t * K, topk_i + t * K, (int)std::min(T - t, kTokens), T, E, K, rule, n_cus, stream);
+        if (rc) return rc;
+    }
+    return MOE_OK;
 }
 
 }  // namespace moe

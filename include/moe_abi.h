@@ -315,7 +315,7 @@ MOE_API int moe_linear_int4(float* y, const void* x, const uint8_t* x_scales, co
 
 /* Load-time repack of an int4 matrix: codes [rows, K / 2] u8 (low half of a byte = even element), scales [rows, ceil(K / group)] bf16, zeros
  * [rows, ceil(K / group)] u8 (low four bits) or NULL (then tiled_zeros is not written and may be NULL) -> the layout moe_linear_int4 reads.
- * moe_int4_tiled_bytes gives the three destination sizes (0 for sizes that the repack rejects).  K % 32 == 0; codes 4-byte aligned, tiled
+ * moe_int4_tiled_bytes gives the three destination sizes (0 for sizes that the repack rejects).  K % 32 == 0; rows, K < 2^31 - 255; codes 4-byte aligned, tiled
  * tensors 16-byte. */
 MOE_API void moe_int4_tiled_bytes(int rows, int K, int group, size_t* code_bytes, size_t* scale_bytes, size_t* zero_bytes);
 MOE_API int moe_int4_repack(const uint8_t* codes, const moe_bf16_t* scales, const uint8_t* zeros, int rows, int K, int group,

@@ -13,3 +13,10 @@ def test_logits_longer_than_the_rows_have_room_of_their_own(pkg):
     """64 experts' rows of one bf16 and one fp32 row a token against 128 and 1024 logits: T * E * 4 bytes more."""
     assert pkg.block_workspace_bytes(8, 64, 64, 128, 1) == 18688 + 8 * 128 * 4
     assert pkg.block_workspace_bytes(500, 64, 64, 1024, 1) == 4392448 + 500 * 1024 * 4
+
+
+def test_int4_sizes_past_32_bits(pkg):
+    """More than 64 GiB of codes; rows and lengths that whole tiles take past 32 bits are refused."""
+    assert pkg.int4_tiled_bytes(1 << 26, 4096, 128) == ((1 << 26) * 2048, (1 << 26) * 64, (1 << 26) * 32)
+    assert pkg.int4_tiled_bytes(0x7FFFFF01, 128, 128) == pkg.int4_tiled_bytes(16, 0x7FFFFF20, 128) == (0, 0, 0)
+    assert pkg.lib.moe_int4_repack(16, 16, None, 0x7FFFFF01, 64, 32, 16, 16, None, None) == -3
