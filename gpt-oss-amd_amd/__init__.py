@@ -176,14 +176,16 @@ def _ptr(t):
     return t.data_ptr()
 
 
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# What torch.cuda asks itself; where torch has neither by these names, its public functions.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _device():
     """Index of the current device; without one an index that no tensor has."""
     try:
         return _current_device()
-    except RuntimeError:
+    except (RuntimeError, AssertionError):  # no device; a torch built without them
         return -2
 
 
