@@ -202,6 +202,16 @@ def _arg(name, t, dtype, n, dev):
     return t.data_ptr()
 
 
+_e4m3, _e8m0 = torch.float8_e4m3fn, getattr(torch, "float8_e8m0fnu", None)
+
+
+def _bytes_arg(name, t, also, n, dev):
+    """_arg for n bytes: uint8, or the 8-bit type that the bytes stand for."""
+    if t is not None and t.dtype is also:
+        t = t.view(_u8)
+    return _arg(name, t, _u8, n, dev)
+
+
 # torch.cuda.current_stream() makes a stream object on every call: 2.9 us, as much as a launch; the handle alone 0.2
 def _stream(stream, dev=None):
     if stream is None:
@@ -392,13 +402,15 @@ def rmsnorm(o, x, weight, batch, size, stream=None):
 def add_rmsnorm(x_out, x, weight, batch, size, delta=None, eps=1e-5, o=None, o_bf16=None, q=None, q_scales=None, q_group=MOE_Q_GROUP_MX,
                 stream=None):
     """x_out = x + delta and its RMSNorm as fp32 (o), bf16 (o_bf16) or e4m3 codes with scales (q, q_scales): moe_add_rmsnorm in
-    include/moe_abi.h.  q_scales: uint8 [batch, size / 32] for q_group 32, float32 [batch, ceil(size / 128)] for 128, [batch] for 0."""
+    include/moe_abi.h.  q: uint8 or float8_e4m3fn.  q_scales: uint8 or float8_e8m0fnu [batch, size / 32] for q_group 32, float32
+    [batch, ceil(size / 128)] for 128, [batch] for 0."""
     n, dev = batch * size, _device()
     n_scales = batch * (1 if q_group == 0 else -(-size // q_group))
+    scales = (_bytes_arg("q_scales", q_scales, _e8m0, n_scales, dev) if q_group == MOE_Q_GROUP_MX
+              else _arg("q_scales", q_scales, _f32, n_scales, dev))
     rc = _lib.moe_add_rmsnorm(_arg("x_out", x_out, _f32, n, dev), _arg("x", x, _f32, n, dev), _arg("delta", delta, _f32, n, dev),
                               _arg("weight", weight, _bf16, size, dev), batch, size, eps, _arg("o", o, _f32, n, dev),
-                              _arg("o_bf16", o_bf16, _bf16, n, dev), _arg("q", q, _u8, n, dev),
-                              _arg("q_scales", q_scales, _u8 if q_group == MOE_Q_GROUP_MX else _f32, n_scales, dev), q_group, _stream(stream, dev))
+                              _arg("o_bf16", o_bf16, _bf16, n, dev), _bytes_arg("q", q, _e4m3, n, dev), scales, q_group, _stream(stream, dev))
     if rc:
         raise MoeError("moe_add_rmsnorm", rc)
 
@@ -407,12 +419,12 @@ def add_rmsnorm(x_out, x, weight, batch, size, delta=None, eps=1e-5, o=None, o_b
 def _linear_rows(x, x_scales, B, K, dev):
     if x_scales is None:
         return _arg("x", x, _bf16, B * K, dev), None
-    return _arg("x", x, _u8, B * K, dev), _arg("x_scales", x_scales, _u8, B * K // 32, dev)
+    return _bytes_arg("x", x, _e4m3, B * K, dev), _bytes_arg("x_scales", x_scales, _e8m0, B * K // 32, dev)
 
 
 def linear_mxfp4(y, x, tiled_blocks, tiled_scales, B, K, N, bias=None, x_scales=None, stream=None):
-    """y [B, N] = x [B, K] W^T + bias for MXFP4 weights (mxfp4_repack of one [1, N, K / 32] tensor); x bf16, or uint8 e4m3 codes with their
-    e8m0 scales [B, K / 32]: moe_linear_mxfp4 in include/moe_abi.h."""
+    """y [B, N] = x [B, K] W^T + bias for MXFP4 weights (mxfp4_repack of one [1, N, K / 32] tensor); x bf16, or e4m3 codes with their
+    e8m0 scales [B, K / 32], each as uint8 or in torch's type for them: moe_linear_mxfp4 in include/moe_abi.h."""
     dev = _device()
     xp, xs = _linear_rows(x, x_scales, B, K, dev)
     rc = _lib.moe_linear_mxfp4(_arg("y", y, _f32, B * N, dev), xp, xs, _arg("tiled_blocks", tiled_blocks, _u8, N * K // 2, dev),
