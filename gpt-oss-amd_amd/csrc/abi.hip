@@ -1019,6 +1019,7 @@ int moe_block_describe(const moe_block_params* caller, char* text, size_t text_b
     const BlockRoute route(p, device_cu_count());
     const bool prefill = route.prefill, direct = route.direct;
     const char* router = "";
+    const bool lanes = !p->route || route_fits_lanes(E, std::max(1, std::min((int)p->route->n_groups, E)));
     switch (route.router) {
         case Router::kScores: router = "router_scores_kernel"; break;
         case Router::kRows: router = "router_rows_kernel"; break;
@@ -1026,8 +1027,13 @@ int moe_block_describe(const moe_block_params* caller, char* text, size_t text_b
         case Router::kFused: router = "router_fused_kernel"; break;
         case Router::kScoresFinalize: router = "router_scores_kernel + router_finalize_kernel"; break;
         case Router::kPartialFinalize: router = "router_partial_kernel + router_finalize_kernel"; break;
-        case Router::kScoresRule: router = "router_scores_kernel + route_kernel"; break;
-        case Router::kPartialRule: router = "router_partial_kernel + router_finalize_kernel + route_kernel"; break;
+        case Router::kScoresRule:
+            router = lanes ? "router_scores_kernel + route_kernel" : "router_scores_kernel + route_any_kernel";
+            break;
+        case Router::kPartialRule:
+            router = lanes ? "router_partial_kernel + router_finalize_kernel + route_kernel"
+                           : "router_partial_kernel + router_finalize_kernel + route_any_kernel";
+            break;
     }
     const int tile_tokens = tile_tokens_of(prefill, fmt);
     BlockWorkspace ws(nullptr, T, H, I, E, K);

@@ -49,6 +49,7 @@ struct RouteRule {  // moe_route_params
     int scoring, n_groups, groups_per_token, group_top, renormalize;
     float scale;
 };
+bool route_fits_lanes(int E, int n_groups);  // route_kernel rather than route_any_kernel
 int launch_route(const float* logits, float* topk_v, int* topk_i, int T, int E, int K, const RouteRule& rule, int n_cus,
                  hipStream_t stream);
 

@@ -469,6 +469,14 @@ __global__ __launch_bounds__(256) void route_any_kernel(const float* __restrict_
     }
 }
 
+// Lanes of a group (log2), where `lpt` lanes share a token.
+static int group_lanes_log(int G, int lpt) {
+    int log = 0;
+    while (G << (log + 1) <= lpt) ++log;
+    return log;
+}
+bool route_fits_lanes(int E, int n_groups) { return ceil_div(E / n_groups, 1 << group_lanes_log(n_groups, 64)) <= 16; }
+
 // Tokens T of a batch of `total`, which is what the lanes of a token go by.
 static int launch_route_part(const float* logits, float* topk_v, int* topk_i, int T, int total, int E, int K, const RouteRule& rule, int n_cus,
                              hipStream_t stream) {
@@ -481,9 +489,8 @@ static int launch_route_part(const float* logits, float* topk_v, int* topk_i, in
     while (lanes < 64 && (long long)total * lanes < 192LL * n_cus) lanes *= 2;
     for (int lpt = lanes; lpt <= 64; lpt *= 2) {
         RouteCut cut;
-        cut.log_group_lanes = 0;
-        while (G << (cut.log_group_lanes + 1) <= lpt) ++cut.log_group_lanes;
         if (G > lpt) continue;
+        cut.log_group_lanes = group_lanes_log(G, lpt);
         cut.group_size = size;
         cut.per_lane = ceil_div(size, 1 << cut.log_group_lanes);
         if (cut.per_lane > 16) continue;
