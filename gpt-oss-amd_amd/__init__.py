@@ -269,7 +269,7 @@ class RouteRule:
     def __init__(self, scoring="softmax", balance_bias=None, n_groups=1, groups_per_token=1, group_top=1, renormalize=True, scale=1.0):
         if scoring not in ("softmax", "sigmoid"):
             raise ValueError("scoring: expected softmax or sigmoid, got %r" % (scoring,))
-        self.balance_bias = balance_bias  # kept alive: the parameters hold its address
+        self.balance_bias = balance_bias
         self.params = RouteParams(struct_bytes=ctypes.sizeof(RouteParams),
                                   scoring={"softmax": MOE_ROUTE_SOFTMAX, "sigmoid": MOE_ROUTE_SIGMOID}[scoring], n_groups=n_groups,
                                   groups_per_token=groups_per_token, group_top=group_top, renormalize=bool(renormalize), scale=scale)
@@ -278,6 +278,7 @@ class RouteRule:
     def of(self, num_experts):
         """The parameters for a call with that many experts."""
         self.params.balance_bias = _arg("balance_bias", self.balance_bias, torch.float32, num_experts, _device())
+        self.held = self.balance_bias  # the parameters hold its address, also those of a prepared block
         return self.ref
 
 
@@ -570,6 +571,7 @@ class MoeBlock:
         if self.route is not None:
             self.route.of(self.E)
             p.route = ctypes.addressof(self.route.params)
+            p.rule = self.route  # lives as long as the block that has its address
         return p
 
     def forward(self, t, e_agg=None, topk_i=None, topk_v=None, router_score=None, residual_x=None, flags=0,
@@ -615,6 +617,7 @@ def pack_layer_params(params):
     arr = (BlockParams * len(params))()
     for i, p in enumerate(params):
         ctypes.memmove(ctypes.byref(arr, i * ctypes.sizeof(BlockParams)), ctypes.byref(p), ctypes.sizeof(BlockParams))
+    arr.rules = [getattr(p, "rule", None) for p in params]  # the copies hold their addresses
     return arr
 
 
