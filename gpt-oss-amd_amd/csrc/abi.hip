@@ -300,6 +300,7 @@ static RouteRule route_rule(const moe_route_params* r) {
 int moe_route(float* topk_values, int* topk_indices, const float* router_logits, int batch_size, int num_experts,
               int experts_per_token, const moe_route_params* rule, moe_stream_t stream) {
     if (!topk_values || !topk_indices || !router_logits || !rule) return MOE_ERR_NULL;
+    if (((uintptr_t)topk_values | (uintptr_t)topk_indices | (uintptr_t)router_logits) & 3u) return MOE_ERR_ALIGN;
     if (batch_size <= 0) return MOE_ERR_SHAPE;
     if (batch_size > kMostRows) return MOE_ERR_LIMIT;
     const int rc = check_route(rule, num_experts, experts_per_token);

@@ -1,4 +1,5 @@
 """What a routing rule's address stands in keeps the rule."""
+import ctypes
 import gc
 import weakref
 
@@ -49,3 +50,9 @@ def test_a_rule_keeps_the_bias_that_its_parameters_hold(pkg, monkeypatch):
     rule.of(8)
     gc.collect()
     assert first() is None and rule.params.balance_bias == rule.balance_bias.data_ptr()
+
+
+def test_route_refuses_addresses_between_values(pkg):
+    rule = ctypes.byref(pkg.RouteParams(struct_bytes=ctypes.sizeof(pkg.RouteParams), n_groups=1, groups_per_token=1, group_top=1))
+    for bad in ((2, 16, 16), (16, 2, 16), (16, 16, 2)):
+        assert pkg.lib.moe_route(*bad, 4, 32, 4, rule, None) == -6
