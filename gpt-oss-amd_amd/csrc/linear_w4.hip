@@ -17,7 +17,7 @@ constexpr int max_waves(int group, int nt) {
     return group == 32 ? 8 : group == 64 ? 12 : 16;
 }
 
-// e4m3 values times a power of two, to bf16 (exact: three mantissa bits).
+// e4m3 values times a power of two (its exponent counts: the bits of 0 are 2^-127), to bf16: exact, with three mantissa bits, but for denormals.
 MOE_DEVICE u32x4 e4m3x8_to_bf16(uint32_t lo, uint32_t hi, float scale) {
     u32x4 v;
     v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));

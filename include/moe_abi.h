@@ -298,12 +298,13 @@ MOE_API int moe_add_rmsnorm(float* x_out, const float* x, const float* delta, co
  * ---------------------------------------------------------------------------------------- */
 
 /* y[b, n] = bias[n] + sum_k x[b, k] W[n, k], fp32 sums, for B rows and an N x K matrix; made for decode-sized batches (the weights are read
- * once per 64 rows).  x [B, K] is bf16 (x_scales NULL) or e4m3 codes with x_scales [B, K / 32] e8m0 as moe_add_rmsnorm writes them (byte 0
- * counts as a factor of 0, as in weights).  bias [N] bf16 or NULL.  K % 32 == 0, K <= 2^24, N <= 2^26, B <= 65535; x and the tiled tensors 16-byte
+ * once per 64 rows).  x [B, K] is bf16 (x_scales NULL) or e4m3 codes with x_scales [B, K / 32] e8m0 as moe_add_rmsnorm writes them: byte b
+ * is 2^(b - 127), 255 a NaN.  Their products become bf16, which is exact from 2^-126 to 2^128; below they are rounded to steps of 2^-133, past
+ * it they are infinities.  bias [N] bf16 or NULL.  K % 32 == 0, K <= 2^24, N <= 2^26, B <= 65535; x and the tiled tensors 16-byte
  * aligned.
  * Deterministic, and a row's result does not depend on the rows around it.
  *
- * moe_linear_mxfp4: tiled_blocks / tiled_scales of moe_mxfp4_repack(E = 1, rows = N, K); N % 64 == 0.
+ * moe_linear_mxfp4: tiled_blocks / tiled_scales of moe_mxfp4_repack(E = 1, rows = N, K), scale bytes 1 to 254; N % 64 == 0.
  *
  * moe_linear_int4: W[n, k] = (code - zero) * scale, codes 0..15, one bf16 scale and one zero point 0..15 for every `group` (32, 64 or 128) values of a
  * row, the last group of which may be shorter; any N.  tiled_* come from moe_int4_repack; tiled_zeros NULL: zero points of 8.  code - zero is
