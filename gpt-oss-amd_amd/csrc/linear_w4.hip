@@ -488,13 +488,13 @@ static int launch_linear_rows(const LinearArgs& a, int n_cus, hipStream_t stream
     const int n_units = ceil_div(a.K, kUnit);
     const long long tiles = (long long)ceil_div(a.N, 16) * ceil_div(a.B, 16 * NT);
     // Blocks of a tile that are there at once, 24 waves of them to a compute unit, up to three: us, so : the first form below, 7 rows of 5760 x 2880 with int4
-    // scales per 64 6.6 : 7.1, 16 rows of 8192 x 1024 4.4 : 4.9, 8 rows of 12288 x 512 int4 3.8 : 5.4.  Not with more of them than that (16 rows of 12288 x
+    // scales per 64 6.5 : 7.1, 16 rows of 8192 x 1024 4.4 : 4.9, 8 rows of 12288 x 512 int4 4.1 : 5.5.  Not with more of them than that (16 rows of 12288 x
     // 4096 12.3 : 11.5, of 8192 x 8192 16.0 : 13.4), nor with more than three, which read x that much more often (16 rows of 16384 x 1536 7.7 : 6.3), nor
     // with 32 rows (64 rows of 5760 x 2880 12.4 : 9.1).
     const int at_once = NT == 1 ? std::clamp(24 / n_units, 1, 3) : 1;
     if (tiles <= (long long)n_cus * at_once && linear_tile_lds(GROUP, NT, n_units) <= kLdsMost) return launch_linear_tile<GROUP, NT>(a, n_units, stream);
     // With up to three tiles to a block the longer ring and the wider steps of the second form cost more code than they hide: us, first : second
-    // form, 64 rows of 5760 x 2880 int4 10.6 : 11.1, 1 row of 16384 x 4096 MXFP4 11.7 : 10.1, 16 rows of 131072 x 2880 42.7 : 38.6.  int4 scales per 32 need the registers of a ring of two for more waves (65536 x 2880, 16 rows, 16 waves : 12 with the ring, 32.3 : 37.4).
+    // form, 16 rows of 6144 x 8192 int4 15.7 : 19.7, 1 row of 16384 x 4096 MXFP4 11.7 : 10.1, 16 rows of 131072 x 2880 42.7 : 38.6.  int4 scales per 32 need the registers of a ring of two for more waves (65536 x 2880, 16 rows, 16 waves : 12 with the ring, 32.3 : 37.4).
     if (tiles <= 3LL * n_cus || GROUP == 32) return launch_linear_of<GROUP, NT, 1, 2>(a, n_cus, stream);
     if constexpr (GROUP != 32) return launch_linear_of<GROUP, NT, 2, 4 / NT>(a, n_cus, stream);
     return MOE_ERR_LIMIT;

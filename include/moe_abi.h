@@ -297,8 +297,8 @@ MOE_API int moe_add_rmsnorm(float* x_out, const float* x, const float* delta, co
  * which holds all its weights in bf16)
  * ---------------------------------------------------------------------------------------- */
 
-/* y[b, n] = bias[n] + sum_k x[b, k] W[n, k], fp32 sums, for B rows and an N x K matrix; made for decode-sized batches (the weights are read
- * once per 64 rows).  x [B, K] is bf16 (x_scales NULL) or e4m3 codes with x_scales [B, K / 32] e8m0 as moe_add_rmsnorm writes them: byte b
+/* y[b, n] = bias[n] + sum_k x[b, k] W[n, k], fp32 sums, for B rows and an N x K matrix; made for decode-sized batches (up to 16 rows go
+ * through the weights together, of more 32 at a time).  x [B, K] is bf16 (x_scales NULL) or e4m3 codes with x_scales [B, K / 32] e8m0 as moe_add_rmsnorm writes them: byte b
  * is 2^(b - 127), 255 a NaN.  Their products become bf16, which is exact from 2^-126 to 2^128; below they are rounded to steps of 2^-133, past
  * it they are infinities.  bias [N] bf16 or NULL.  K % 32 == 0, K <= 2^24, N <= 2^26, B <= 65535; x and the tiled tensors 16-byte
  * aligned.
