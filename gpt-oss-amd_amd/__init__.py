@@ -26,6 +26,8 @@ MOE_FLAG_FORCE_BUCKET_LAUNCH = 16
 MOE_FLAG_FUSED_GEMM_LAUNCH = 32
 MOE_ROUTE_SOFTMAX = 0
 MOE_ROUTE_SIGMOID = 1
+MOE_ROWS_F32 = 0
+MOE_ROWS_BF16 = 1
 MOE_Q_GROUP_ROW = 0
 MOE_Q_GROUP_MX = 32
 MOE_Q_GROUP_128 = 128
@@ -91,6 +93,21 @@ class RouteParams(_c.Structure):
     ]
 
 
+class KvCacheParams(_c.Structure):
+    """moe_kv_cache of include/moe_abi.h."""
+    _fields_ = [
+        ("struct_bytes", _c.c_uint32),
+        ("n_pages", _c.c_int32),
+        ("page_size", _c.c_int32),
+        ("n_kv_heads", _c.c_int32),
+        ("head_dim", _c.c_int32),
+        ("k", _vp),
+        ("v", _vp),
+        ("k_scales", _vp),
+        ("v_scales", _vp),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/moe_abi.h declares
 SIGNATURES = {
     "moe_abi_version": (_i, []),
@@ -107,6 +124,12 @@ SIGNATURES = {
     "moe_linear_int4": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "moe_int4_tiled_bytes": (None, [_i, _i, _i, _c.POINTER(_sz), _c.POINTER(_sz), _c.POINTER(_sz)]),
     "moe_int4_repack": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "moe_rope_kv_write": (_i, [_vp, _i, _ll, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "moe_attention_decode_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "moe_attention_decode": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp, _sz, _vp]),
+    "moe_attention_prefill": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _i, _f, _vp, _vp]),
+    "moe_token_logprobs_workspace_bytes": (_sz, [_i, _i, _i]),
+    "moe_token_logprobs": (_i, [_vp, _i, _ll, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "moe_topk": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
     "moe_softmax": (_i, [_vp, _i, _i, _vp]),
     "moe_bucket_by_expert": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
@@ -470,6 +493,126 @@ def linear_int4(y, x, tiled_codes, tiled_scales, B, K, N, group, tiled_zeros=Non
                               _arg("bias", bias, _bf16, N, dev), B, K, N, group, _stream(stream, dev))
     if rc:
         raise MoeError("moe_linear_int4", rc)
+
+
+# ---- attention and what surrounds it -------------------------------------------------------------
+def _rows_arg(name, t, dtype, rows, width, dev):
+    """(address, elements from row to row) of `rows` rows of `width` values of one type on device `dev`, each row contiguous."""
+    n = t.shape[0] if t.dim() > 1 else 0
+    if t.dtype is not dtype or n < rows or t.numel() != n * width:
+        raise ValueError("%s: expected %d rows of %d values of %s, got %s of %s" % (name, rows, width, dtype, tuple(t.shape), t.dtype))
+    if t.get_device() != dev:
+        raise ValueError("%s: expected a tensor on the current device" % name)
+    if t.is_contiguous():
+        return t.data_ptr(), width
+    if not t[0].is_contiguous():
+        raise ValueError("%s: expected contiguous rows" % name)
+    return t.data_ptr(), t.stride(0)
+
+
+def _rows_type(name, t):
+    if t.dtype is _f32:
+        return MOE_ROWS_F32
+    if t.dtype is _bf16:
+        return MOE_ROWS_BF16
+    raise ValueError("%s: expected torch.float32 or torch.bfloat16, got %s" % (name, t.dtype))
+
+
+class KvCache:
+    """A paged cache (moe_kv_cache): k, v [n_pages, n_kv_heads, page_size, head_dim], bf16, or e4m3 codes (uint8 or float8_e4m3fn) with k_scales, v_scales
+    [n_pages, n_kv_heads, page_size, head_dim / 32] (uint8 or float8_e8m0fnu)."""
+
+    def __init__(self, k, v, k_scales=None, v_scales=None):
+        if k.dim() != 4 or v.shape != k.shape:
+            raise ValueError("k, v: expected [n_pages, n_kv_heads, page_size, head_dim], got %s and %s" % (tuple(k.shape), tuple(v.shape)))
+        if (k_scales is None) != (v_scales is None):
+            raise ValueError("k_scales, v_scales: expected both or neither")
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        dev, n, held = k.get_device(), k.numel(), []
+        if k_scales is None:
+            held = [_arg("k", k, _bf16, n, dev), _arg("v", v, _bf16, n, dev), None, None]
+        else:
+            held = [_bytes_arg("k", k, _e4m3, n, dev), _bytes_arg("v", v, _e4m3, n, dev), _bytes_arg("k_scales", k_scales, _e8m0, n // 32, dev),
+                    _bytes_arg("v_scales", v_scales, _e8m0, n // 32, dev)]
+        self.device = dev
+        self.params = KvCacheParams(ctypes.sizeof(KvCacheParams), self.n_pages, self.page_size, self.n_kv_heads, self.head_dim, *held)
+        self.address = ctypes.addressof(self.params)
+
+    def of(self, dev):
+        """The parameters' address for a call on device `dev`."""
+        if self.device != dev:
+            raise ValueError("cache: expected tensors on the current device")
+        return self.address
+
+
+def rope_kv_write(q, qkv, positions, inv_freq, n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim=None, rope_scale=1.0, k=None, v=None, cache=None,
+                  slots=None, stream=None):
+    """Rows qkv [n_tokens, (n_heads + 2 n_kv_heads) * head_dim] (fp32 or bf16, contiguous rows) -> queries and keys turned by position, as
+    bf16 rows q, k, v and in the cache's slots: moe_rope_kv_write in include/moe_abi.h.  q, k, v, and cache with slots may be None."""
+    dev = _device()
+    rotary_dim = head_dim if rotary_dim is None else rotary_dim
+    rows, stride = _rows_arg("qkv", qkv, _bf16 if qkv.dtype is _bf16 else _f32, n_tokens, (n_heads + 2 * n_kv_heads) * head_dim, dev)
+    i32, nkv = torch.int32, n_tokens * n_kv_heads * head_dim
+    rc = _lib.moe_rope_kv_write(rows, _rows_type("qkv", qkv), stride, _arg("positions", positions, i32, n_tokens, dev),
+                                _arg("inv_freq", inv_freq, _f32, rotary_dim // 2, dev), n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, rope_scale,
+                                _arg("q", q, _bf16, n_tokens * n_heads * head_dim, dev), _arg("k", k, _bf16, nkv, dev), _arg("v", v, _bf16, nkv, dev),
+                                None if cache is None else cache.of(dev), _arg("slots", slots, i32, n_tokens, dev), _stream(stream, dev))
+    if rc:
+        raise MoeError("moe_rope_kv_write", rc)
+
+
+def attention_decode_workspace_bytes(batch, n_heads, n_kv_heads, head_dim):
+    return _lib.moe_attention_decode_workspace_bytes(batch, n_heads, n_kv_heads, head_dim)
+
+
+def attention_decode(out, q, cache, page_table, lengths, batch, n_heads, scale, workspace, window=0, sinks=None, stream=None):
+    """Attention of one query a sequence, q [batch, n_heads, head_dim] bf16, over the pages page_table [batch, max_pages] int32 of a KvCache:
+    moe_attention_decode in include/moe_abi.h.  workspace: uint8, attention_decode_workspace_bytes."""
+    dev = _device()
+    n = batch * n_heads * cache.head_dim
+    if page_table.dim() != 2:
+        raise ValueError("page_table: expected [batch, max_pages], got %s" % (tuple(page_table.shape),))
+    max_pages = page_table.shape[1]
+    rc = _lib.moe_attention_decode(_arg("out", out, _bf16, n, dev), _arg("q", q, _bf16, n, dev), cache.of(dev),
+                                   _arg("page_table", page_table, torch.int32, batch * max_pages, dev), _arg("lengths", lengths, torch.int32, batch, dev),
+                                   batch, n_heads, max_pages, window, scale, _arg("sinks", sinks, _bf16, n_heads, dev),
+                                   _arg("workspace", workspace, _u8, 0, dev), workspace.numel(), _stream(stream, dev))
+    if rc:
+        raise MoeError("moe_attention_decode", rc)
+
+
+def attention_prefill(out, q, k, v, q_starts, k_starts, n_seqs, n_heads, n_kv_heads, head_dim, scale, window=0, sinks=None, stream=None):
+    """Causal attention over packed prompts: q, out [total_q, n_heads, head_dim], k, v [total_k, n_kv_heads, head_dim] bf16, whose tokens may lie
+    further apart than they are long; q_starts, k_starts int32 [n_seqs + 1]: moe_attention_prefill in include/moe_abi.h."""
+    dev = _device()
+    total_q, total_k, i32 = q.shape[0], k.shape[0], torch.int32
+    op, os_ = _rows_arg("out", out, _bf16, total_q, n_heads * head_dim, dev)
+    qp, qs = _rows_arg("q", q, _bf16, total_q, n_heads * head_dim, dev)
+    kp, ks = _rows_arg("k", k, _bf16, total_k, n_kv_heads * head_dim, dev)
+    vp, vs = _rows_arg("v", v, _bf16, total_k, n_kv_heads * head_dim, dev)
+    rc = _lib.moe_attention_prefill(op, qp, kp, vp, _arg("q_starts", q_starts, i32, n_seqs + 1, dev), _arg("k_starts", k_starts, i32, n_seqs + 1, dev), n_seqs,
+                                    total_q, total_k, n_heads, n_kv_heads, head_dim, os_, qs, ks, vs, window, scale,
+                                    _arg("sinks", sinks, _bf16, n_heads, dev), _stream(stream, dev))
+    if rc:
+        raise MoeError("moe_attention_prefill", rc)
+
+
+def token_logprobs_workspace_bytes(n_tokens, vocab, top_k):
+    return _lib.moe_token_logprobs_workspace_bytes(n_tokens, vocab, top_k)
+
+
+def token_logprobs(logits, tokens, n_tokens, vocab, logprobs=None, entropy=None, top_logprobs=None, top_indices=None, top_k=0, workspace=None, stream=None):
+    """Rows of logits [n_tokens, vocab] (fp32 or bf16, contiguous rows) -> log probability of each row's token, entropy, the top_k largest:
+    moe_token_logprobs in include/moe_abi.h.  workspace: uint8, token_logprobs_workspace_bytes, or None where that is 0."""
+    dev, i32 = _device(), torch.int32
+    rows, stride = _rows_arg("logits", logits, _bf16 if logits.dtype is _bf16 else _f32, n_tokens, vocab, dev)
+    rc = _lib.moe_token_logprobs(rows, _rows_type("logits", logits), stride, _arg("tokens", tokens, i32, n_tokens, dev), n_tokens, vocab, top_k,
+                                 _arg("logprobs", logprobs, _f32, n_tokens, dev), _arg("entropy", entropy, _f32, n_tokens, dev),
+                                 _arg("top_logprobs", top_logprobs, _f32, n_tokens * top_k, dev), _arg("top_indices", top_indices, i32, n_tokens * top_k, dev),
+                                 _arg("workspace", workspace, _u8, 0, dev), 0 if workspace is None else workspace.numel(), _stream(stream, dev))
+    if rc:
+        raise MoeError("moe_token_logprobs", rc)
 
 
 # ---- MXFP4 -------------------------------------------------------------------------------------

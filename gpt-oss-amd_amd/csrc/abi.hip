@@ -10,6 +10,7 @@
 #include <cstddef>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <new>
 
 using namespace moe;
@@ -600,6 +601,130 @@ int moe_int4_repack(const uint8_t* codes, const moe_bf16_t* scales, const uint8_
     if (((uintptr_t)codes & 3u) || ((uintptr_t)scales & 1u)) return MOE_ERR_ALIGN;
     if (((uintptr_t)tiled_codes | (uintptr_t)tiled_scales | (uintptr_t)tiled_zeros) & 15u) return MOE_ERR_ALIGN;
     return launch_int4_repack(codes, scales, zeros, rows, K, group, tiled_codes, tiled_scales, tiled_zeros, as_stream(stream));
+}
+
+// ---- attention and what surrounds it -----------------------------------------------------------
+static inline bool misaligned(std::initializer_list<const void*> pointers, unsigned to) {
+    uintptr_t bits = 0;
+    for (const void* p : pointers) bits |= reinterpret_cast<uintptr_t>(p);
+    return bits & (to - 1);
+}
+static int check_heads(int n_heads, int n_kv_heads, int head_dim) {
+    if (n_heads <= 0 || n_kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return MOE_ERR_SHAPE;
+    if (n_heads > 1024 || n_kv_heads > 1024) return MOE_ERR_LIMIT;
+    return MOE_OK;
+}
+static int check_cache(const moe_kv_cache* c) {
+    if (c->struct_bytes != sizeof(moe_kv_cache)) return MOE_ERR_FORMAT;
+    if (!c->k || !c->v || !c->k_scales != !c->v_scales) return MOE_ERR_NULL;
+    if (c->n_pages <= 0 || c->page_size <= 0 || (c->page_size & (c->page_size - 1)) || c->page_size < 16) return MOE_ERR_SHAPE;
+    if (c->page_size > (1 << 20) || (long long)c->n_pages * c->page_size > 0x7FFFFFFFll) return MOE_ERR_LIMIT;
+    const int rc = check_heads(c->n_kv_heads, c->n_kv_heads, c->head_dim);
+    if (rc) return rc;
+    return misaligned({c->k, c->v}, 16) ? MOE_ERR_ALIGN : MOE_OK;
+}
+static inline int log2_of(int power) { return __builtin_ctz((unsigned)power); }
+static inline bool bad_scale(float scale) { return !(scale > 0.f) || scale > 3.4028234e38f; }
+
+int moe_rope_kv_write(const void* qkv, int qkv_type, long long stride, const int* positions, const float* inv_freq, int n_tokens, int n_heads,
+                      int n_kv_heads, int head_dim, int rotary_dim, float scale, moe_bf16_t* q, moe_bf16_t* k, moe_bf16_t* v,
+                      const moe_kv_cache* cache, const int* slots, moe_stream_t stream) {
+    if (!qkv || (rotary_dim && (!positions || !inv_freq)) || !cache != !slots || (!q && !k && !v && !cache)) return MOE_ERR_NULL;
+    if (qkv_type != MOE_ROWS_F32 && qkv_type != MOE_ROWS_BF16) return MOE_ERR_FORMAT;
+    if (n_tokens <= 0 || rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 8 != 0) return MOE_ERR_SHAPE;
+    int rc = check_heads(n_heads, n_kv_heads, head_dim);
+    if (rc) return rc;
+    if (n_tokens > kMostRows) return MOE_ERR_LIMIT;
+    if (stride < (long long)(n_heads + 2 * n_kv_heads) * head_dim || stride % 4 != 0) return MOE_ERR_SHAPE;
+    if (misaligned({qkv, q, k, v}, 16) || misaligned({positions, inv_freq, slots}, 4)) return MOE_ERR_ALIGN;
+    RopeKvArgs a{qkv, stride, positions, inv_freq, q, k, v, nullptr, nullptr, nullptr, nullptr, slots, n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, 0, 0, scale};
+    if (cache) {
+        rc = check_cache(cache);
+        if (rc) return rc;
+        if (cache->n_kv_heads != n_kv_heads || cache->head_dim != head_dim || (cache->k_scales && rotary_dim % 64 != 0)) return MOE_ERR_SHAPE;
+        a.cache_k = static_cast<uint8_t*>(cache->k);
+        a.cache_v = static_cast<uint8_t*>(cache->v);
+        a.k_scales = cache->k_scales;
+        a.v_scales = cache->v_scales;
+        a.page_shift = log2_of(cache->page_size);
+        a.n_slots = (long long)cache->n_pages * cache->page_size;
+    }
+    return launch_rope_kv_write(a, qkv_type == MOE_ROWS_BF16, as_stream(stream));
+}
+
+static int check_decode(int batch, int n_heads, int n_kv_heads, int head_dim) {
+    const int rc = check_heads(n_heads, n_kv_heads, head_dim);
+    if (rc) return rc;
+    if (batch <= 0 || n_heads % n_kv_heads != 0) return MOE_ERR_SHAPE;
+    return batch > 65535 ? MOE_ERR_LIMIT : MOE_OK;
+}
+
+size_t moe_attention_decode_workspace_bytes(int batch, int n_heads, int n_kv_heads, int head_dim) {
+    size_t ml, o;
+    return check_decode(batch, n_heads, n_kv_heads, head_dim) ? 0 : attention_decode_workspace(batch, n_heads, n_kv_heads, head_dim, &ml, &o);
+}
+
+int moe_attention_decode(moe_bf16_t* out, const moe_bf16_t* q, const moe_kv_cache* cache, const int* page_table, const int* lengths, int batch,
+                         int n_heads, int max_pages, int window, float scale, const moe_bf16_t* sinks, void* workspace, size_t workspace_bytes,
+                         moe_stream_t stream) {
+    if (!out || !q || !cache || !page_table || !lengths) return MOE_ERR_NULL;
+    int rc = check_cache(cache);
+    if (!rc) rc = check_decode(batch, n_heads, cache->n_kv_heads, cache->head_dim);
+    if (rc) return rc;
+    if (max_pages <= 0 || window < 0) return MOE_ERR_SHAPE;
+    if ((long long)max_pages * cache->page_size > (1 << 30)) return MOE_ERR_LIMIT;
+    if (bad_scale(scale)) return MOE_ERR_FORMAT;
+    if (misaligned({out, q}, 16) || misaligned({page_table, lengths}, 4) || misaligned({sinks}, 2)) return MOE_ERR_ALIGN;
+    size_t ml, o;
+    if (!workspace || misaligned({workspace}, 16) || workspace_bytes < attention_decode_workspace(batch, n_heads, cache->n_kv_heads, cache->head_dim, &ml, &o))
+        return MOE_ERR_WORKSPACE;
+    char* ws = static_cast<char*>(workspace);
+    return launch_attention_decode({out, q, cache->k, cache->v, cache->k_scales, cache->v_scales, page_table, lengths, sinks, reinterpret_cast<int*>(ws),
+                                    reinterpret_cast<float*>(ws + ml), reinterpret_cast<float*>(ws + o), batch, n_heads, cache->n_kv_heads, max_pages,
+                                    cache->n_pages, log2_of(cache->page_size), window, scale, 0, 0},
+                                   cache->head_dim, as_stream(stream));
+}
+
+int moe_attention_prefill(moe_bf16_t* out, const moe_bf16_t* q, const moe_bf16_t* k, const moe_bf16_t* v, const int* q_starts, const int* k_starts,
+                          int n_seqs, int total_q, int total_k, int n_heads, int n_kv_heads, int head_dim, long long out_stride, long long q_stride,
+                          long long k_stride, long long v_stride, int window, float scale, const moe_bf16_t* sinks, moe_stream_t stream) {
+    if (!out || !q || !k || !v || !q_starts || !k_starts) return MOE_ERR_NULL;
+    const int rc = check_heads(n_heads, n_kv_heads, head_dim);
+    if (rc) return rc;
+    if (n_seqs <= 0 || total_q <= 0 || total_k <= 0 || n_heads % n_kv_heads != 0 || window < 0) return MOE_ERR_SHAPE;
+    if (std::min(out_stride, q_stride) < (long long)n_heads * head_dim || std::min(k_stride, v_stride) < (long long)n_kv_heads * head_dim) return MOE_ERR_SHAPE;
+    if ((out_stride | q_stride | k_stride | v_stride) % 8 != 0) return MOE_ERR_SHAPE;
+    if (n_seqs > 65535 || (long long)total_q * n_heads >= (1 << 30)) return MOE_ERR_LIMIT;
+    if (bad_scale(scale)) return MOE_ERR_FORMAT;
+    if (misaligned({out, q, k, v}, 16) || misaligned({q_starts, k_starts}, 4) || misaligned({sinks}, 2)) return MOE_ERR_ALIGN;
+    return launch_attention_prefill({out, q, k, v, q_starts, k_starts, sinks, out_stride, q_stride, k_stride, v_stride, n_seqs, total_q, total_k, n_heads,
+                                     n_kv_heads, window, scale},
+                                    head_dim, as_stream(stream));
+}
+
+static int check_logprobs(int n_tokens, int vocab, int top_k) {
+    if (n_tokens <= 0 || vocab <= 0 || top_k < 0 || top_k > vocab) return MOE_ERR_SHAPE;
+    return n_tokens > kMostRows || vocab > (1 << 30) || top_k > 32 ? MOE_ERR_LIMIT : MOE_OK;
+}
+
+size_t moe_token_logprobs_workspace_bytes(int n_tokens, int vocab, int top_k) {
+    return check_logprobs(n_tokens, vocab, top_k) ? 0 : logprob_workspace(n_tokens, vocab, top_k);
+}
+
+int moe_token_logprobs(const void* logits, int logits_type, long long stride, const int* tokens, int n_tokens, int vocab, int top_k, float* logprobs,
+                       float* entropy, float* top_logprobs, int* top_indices, void* workspace, size_t workspace_bytes, moe_stream_t stream) {
+    if (!logits || (!logprobs && !entropy && !top_logprobs) || (logprobs && !tokens)) return MOE_ERR_NULL;
+    if (!top_logprobs != !top_indices || !top_logprobs != !top_k) return MOE_ERR_NULL;
+    if (logits_type != MOE_ROWS_F32 && logits_type != MOE_ROWS_BF16) return MOE_ERR_FORMAT;
+    const int rc = check_logprobs(n_tokens, vocab, top_k);
+    if (rc) return rc;
+    if (stride < vocab) return MOE_ERR_SHAPE;
+    const bool bf16 = logits_type == MOE_ROWS_BF16;
+    if (misaligned({logits}, bf16 ? 2 : 4) || misaligned({tokens, logprobs, entropy, top_logprobs, top_indices}, 4)) return MOE_ERR_ALIGN;
+    const size_t need = logprob_workspace(n_tokens, vocab, top_k);
+    if (need && (!workspace || misaligned({workspace}, 16) || workspace_bytes < need)) return MOE_ERR_WORKSPACE;
+    return launch_token_logprobs({logits, stride, tokens, logprobs, entropy, top_logprobs, top_indices, workspace, n_tokens, vocab, top_k}, bf16,
+                                 as_stream(stream));
 }
 
 // ---- MXFP4 -----------------------------------------------------------------------------------

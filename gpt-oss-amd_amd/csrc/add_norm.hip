@@ -4,39 +4,12 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "mx8.h"
 #include "norm.h"
 
 namespace moe {
 
-namespace {
-
-MOE_DEVICE uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-
-// Bits of the largest |value| (those of an infinity or a NaN are above all others).
-MOE_DEVICE uint32_t amax_bits(const float4& y) {
-    return max(max(abs_bits(y.x), abs_bits(y.y)), max(abs_bits(y.z), abs_bits(y.w)));
-}
-// The largest |value| before the rounding to fp32; what is not finite the bits above tell.
-MOE_DEVICE double amax_of(const Double4& y) { return fmax(fmax(fabs(y.x), fabs(y.y)), fmax(fabs(y.z), fabs(y.w))); }
-
-// Maximum over groups of LANES (8, 32 or 64) neighbouring lanes, in all of them.
-template <int LANES>
-MOE_DEVICE uint32_t group_max(uint32_t v) {
-    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true));   // lanes that differ in bit 0,
-    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true));   // bit 1,
-    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true));  // mirrored in 8 lanes,
-    if constexpr (LANES > 8) {
-        v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true));  // in 16,
-        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);             // neighbouring rows,
-        v = max(r[0], r[1]);
-    }
-    if constexpr (LANES > 32) {
-        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);  // halves
-        v = max(r[0], r[1]);
-    }
-    return v;
-}
-// The same of doubles that are not negative and not NaN: their bits are in their order.
+// group_max of doubles that are not negative and not NaN: their bits are in their order.
 template <int LANES>
 MOE_DEVICE double group_max(double v) {
     const uint32_t hi = (uint32_t)(__builtin_bit_cast(uint64_t, v) >> 32), lo = (uint32_t)__builtin_bit_cast(uint64_t, v);
@@ -45,13 +18,14 @@ MOE_DEVICE double group_max(double v) {
     return __builtin_bit_cast(double, ((uint64_t)most << 32) | rest);
 }
 
-// Power-of-two scale of a group (e8m0): the smallest 2^(b - 127), b >= 1, that brings its largest value to 448 or below.  448 = 1.75 * 2^8, so
-// the exponent field goes up by one where the mantissa is past 1.75.  255 where the group holds an infinity or a NaN.
-MOE_DEVICE uint32_t mx_scale_byte(uint32_t amax) {
-    if (amax >= 0x7F800000u) return 255u;
-    const int b = (int)((amax + 0x1FFFFFu) >> 23) - 8;
-    return (uint32_t)max(b, 1);
+namespace {
+
+// Bits of the largest |value| (those of an infinity or a NaN are above all others).
+MOE_DEVICE uint32_t amax_bits(const float4& y) {
+    return max(max(abs_bits(y.x), abs_bits(y.y)), max(abs_bits(y.z), abs_bits(y.w)));
 }
+// The largest |value| before the rounding to fp32; what is not finite the bits above tell.
+MOE_DEVICE double amax_of(const Double4& y) { return fmax(fmax(fabs(y.x), fabs(y.y)), fmax(fabs(y.z), fabs(y.w))); }
 
 // fp32 scale of a group of largest |value| amax (bits: in fp32), and what its values are multiplied by: 448 / amax to 2^-48.
 MOE_DEVICE void f32_scale(uint32_t bits, double amax, float& scale, double& mult) {

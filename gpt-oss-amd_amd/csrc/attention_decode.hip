@@ -1,0 +1,356 @@
+// Attention of one query row a sequence over a paged key-value cache: out = softmax(scale q K^T, sinks) V.
+#include <algorithm>
+
+#include "attention.h"
+#include "kernels.h"
+#include "mx8.h"
+
+namespace moe {
+
+namespace {
+
+constexpr int kWaves = 4, kTile = 32;  // waves of a block; keys that a wave takes at a time
+
+// What a sequence's query sees: keys first .. len - 1, counted from the tile that holds the first of them.
+struct Seen {
+    int first, len, start;
+    MOE_DEVICE int keys() const { return len - start; }
+};
+MOE_DEVICE Seen seen_of(const AttentionDecodeArgs& a, int b) {
+    const long long room = (long long)a.max_pages << a.page_shift;
+    const int len = (int)min((long long)max(a.lengths[b], 0), room);
+    const int first = a.window ? max(0, len - a.window) : 0;
+    return {first, len, first & ~(kTile - 1)};
+}
+
+// A wave's tile in the registers, as it comes: whole rows, 16 bytes to a lane.
+template <int D, bool MX>
+struct TileLoads {
+    static constexpr int kRowBytes = MX ? D : 2 * D, kLanes = kRowBytes / 16, kRows = 64 / kLanes, kLoads = kTile / kRows;
+    u32x4 k[kLoads], v[kLoads];
+    uint32_t ks[MX ? kLoads : 1], vs[MX ? kLoads : 1];
+    bool valid[2];  // whether the pages of keys 0 .. 15 and 16 .. 31 exist
+};
+
+// Scale byte of 32 values: 2^(b - 127), 255 a NaN.
+MOE_DEVICE float mx_scale(uint32_t b) { return __uint_as_float(b == 255u ? 0x7FC00000u : b << 23); }
+
+}  // namespace
+
+// Item (sequence, piece of its keys, KV head, 16 of the query heads that share it) to a block; pieces are as long as makes about a.pieces of
+// them per head over all sequences, so that the longest sequence does not hold up the others.  A wave takes every fourth tile of 32 keys:
+// whole rows of K and V into registers a tile ahead, through its own LDS into the matrix operands.  S^T = K Q^T puts a query head into
+// a lane column, so that its running maximum and sum are a lane's and P^T is the second product's operand as it stands: O^T = V^T P^T, with
+// V^T read as columns from LDS.  P is rounded to bf16 for that product (half a step is up to 2^-8 of a weight, as that of the bf16 result); its sum is
+// taken before that, in fp32.  Statistics are in powers of two: s' = scale log2(e) q.k.
+template <int D, bool MX>
+__global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(AttentionDecodeArgs a) {
+    constexpr int kRow = 2 * D, kSteps = D / 32, kDims = D / 16;
+    using Loads = TileLoads<D, MX>;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane & 15, g = lane >> 4;
+    const int G = a.n_heads / a.n_kv_heads, group_tiles = ceil_div(G, 16);
+    const int h = blockIdx.x % a.n_kv_heads, rest = blockIdx.x / a.n_kv_heads, gt = rest % group_tiles, item = rest / group_tiles;
+
+    // the piece
+    double total = 0.0;  // keys of all sequences, exact
+    for (int base = 0; base < a.batch; base += 64) total += wave_sum(base + lane < a.batch ? (double)seen_of(a, base + lane).keys() : 0.0);
+    const long long even = (long long)(total / a.pieces) + 1;
+    const int piece = (int)min(max((even + kTile - 1) / kTile * kTile, (long long)a.min_piece), 1ll << 30);
+    int b, part;
+    auto pieces_of = [&](int s) { return max(1, ceil_div(seen_of(a, s).keys(), piece)); };
+    if (!find_item(a.batch, item, pieces_of, b, part)) return;
+    const Seen seen = seen_of(a, b);
+    const int n_parts = max(1, ceil_div(seen.keys(), piece));
+    const int begin = seen.start + part * piece, end = min(seen.len, begin + piece);
+
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * 2 * kTile * kRow];
+    uint8_t* k_lds = lds + wave * 2 * kTile * kRow;
+    uint8_t* v_lds = k_lds + kTile * kRow;
+
+    u32x4 qf[kSteps];
+    {
+        const int head = 16 * gt + q;
+        const uint16_t* row = a.q + ((size_t)b * a.n_heads + (size_t)h * G + min(head, G - 1)) * D;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            qf[s] = *reinterpret_cast<const u32x4*>(row + 32 * s + 8 * g);
+            if (head >= G) qf[s] = u32x4{0, 0, 0, 0};
+        }
+    }
+
+    // page numbers, 64 at a time, a lane to each
+    const int* table = a.page_table + (size_t)b * a.max_pages;
+    int pages_from = -64, pages = 0;
+    auto page_at = [&](int key) {
+        const int at = key >> a.page_shift;
+        if (at - pages_from >= 64) {
+            pages_from = at;
+            pages = at + lane < a.max_pages ? table[at + lane] : -1;
+        }
+        return __builtin_amdgcn_readlane(pages, at - pages_from);
+    };
+    auto load = [&](Loads& t, int key0) {
+        const uint8_t* kp[2];
+        const uint8_t* vp[2];
+        const uint8_t* ksp[2];
+        const uint8_t* vsp[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int key = key0 + 16 * i;
+            const int page = key < end ? page_at(key) : -1;
+            t.valid[i] = (unsigned)page < (unsigned)a.n_pages;
+            const size_t row = ((size_t)(t.valid[i] ? page : 0) * a.n_kv_heads + h) << a.page_shift | (size_t)(key & ((1 << a.page_shift) - 1));
+            kp[i] = static_cast<const uint8_t*>(a.k) + row * Loads::kRowBytes;
+            vp[i] = static_cast<const uint8_t*>(a.v) + row * Loads::kRowBytes;
+            if constexpr (MX) {
+                ksp[i] = a.k_scales + row * (D / 32);
+                vsp[i] = a.v_scales + row * (D / 32);
+            }
+        }
+        const int r = lane / Loads::kLanes, c = lane % Loads::kLanes;
+#pragma unroll
+        for (int i = 0; i < Loads::kLoads; ++i) {
+            const int half = i * Loads::kRows / 16, at = i * Loads::kRows % 16 + r;
+            t.k[i] = *reinterpret_cast<const u32x4*>(kp[half] + at * Loads::kRowBytes + 16 * c);
+            t.v[i] = *reinterpret_cast<const u32x4*>(vp[half] + at * Loads::kRowBytes + 16 * c);
+            if constexpr (MX) {
+                t.ks[i] = ksp[half][at * (D / 32) + c / 2];
+                t.vs[i] = vsp[half][at * (D / 32) + c / 2];
+            }
+        }
+    };
+
+    f32x4 acc[kDims];
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    const float scale = a.scale * kLog2e;
+
+    auto compute = [&](Loads& t, int key0) {
+        const bool whole = key0 >= seen.first && key0 + kTile <= end && t.valid[0] && t.valid[1];
+        auto visible = [&](int key) { return key >= seen.first && key < end && t.valid[(key - key0) >> 4]; };
+        // to LDS: 16-byte chunk c of row r at c ^ (r % 8) for K, which is read by rows, at c ^ 2 (r % 4) for V, read by columns of four rows
+        const int r0 = lane / Loads::kLanes, c = lane % Loads::kLanes;
+#pragma unroll
+        for (int i = 0; i < Loads::kLoads; ++i) {
+            const int r = i * Loads::kRows + r0;
+            if (!whole && !visible(key0 + r)) t.v[i] = u32x4{0, 0, 0, 0};  // a weight of 0 does not undo a NaN
+            uint8_t* kr = k_lds + r * kRow;
+            uint8_t* vr = v_lds + r * kRow;
+            const int ks = r & 7, vs = (r & 3) << 1;
+            if constexpr (MX) {
+                const float k_scale = mx_scale(t.ks[i]), v_scale = !whole && !visible(key0 + r) ? 1.f : mx_scale(t.vs[i]);
+                *reinterpret_cast<u32x4*>(kr + ((2 * c) ^ ks) * 16) = e4m3x8_to_bf16(t.k[i][0], t.k[i][1], k_scale);
+                *reinterpret_cast<u32x4*>(kr + ((2 * c + 1) ^ ks) * 16) = e4m3x8_to_bf16(t.k[i][2], t.k[i][3], k_scale);
+                *reinterpret_cast<u32x4*>(vr + ((2 * c) ^ vs) * 16) = e4m3x8_to_bf16(t.v[i][0], t.v[i][1], v_scale);
+                *reinterpret_cast<u32x4*>(vr + ((2 * c + 1) ^ vs) * 16) = e4m3x8_to_bf16(t.v[i][2], t.v[i][3], v_scale);
+            } else {
+                *reinterpret_cast<u32x4*>(kr + (c ^ ks) * 16) = t.k[i];
+                *reinterpret_cast<u32x4*>(vr + (c ^ vs) * 16) = t.v[i];
+            }
+        }
+        lds_in_order();
+        f32x4 s[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                const int r = 16 * i + q;
+                s[i] = mfma_16x16x32(*reinterpret_cast<const u32x4*>(k_lds + r * kRow + ((4 * j + g) ^ (r & 7)) * 16), qf[j], s[i]);
+            }
+        }
+        settle(s[0], s[1]);
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[i][j] *= scale;
+                if (!whole && !visible(key0 + 16 * i + 4 * g + j)) s[i][j] = -INFINITY;
+                most = fmaxf(most, s[i][j]);
+            }
+        most = fmaxf(m, max_of_groups(most));
+        const float base = most == -INFINITY ? 0.f : most;
+        const float down = __builtin_amdgcn_exp2f(m - base);  // nothing so far: 0
+        m = most;
+        l *= down;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) acc[d] *= down;
+        u32x4 p;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[i][j] = __builtin_amdgcn_exp2f(s[i][j] - base);
+                l += s[i][j];
+            }
+            p[2 * i] = pack_bf16x2(s[i][0], s[i][1]);
+            p[2 * i + 1] = pack_bf16x2(s[i][2], s[i][3]);
+        }
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) {
+            u32x2 col[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = 16 * i + 4 * g + (q >> 2);
+                col[i] = lds_column_of_4(v_lds + r * kRow + ((2 * d + ((q & 3) >> 1)) ^ ((r & 3) << 1)) * 16 + (q & 1) * 8);
+            }
+            acc[d] = mfma_16x16x32(u32x4{col[0][0], col[0][1], col[1][0], col[1][1]}, p, acc[d]);
+        }
+        lds_in_order();
+    };
+
+    const int step = kWaves * kTile;
+    int key0 = begin + wave * kTile;
+    if (key0 < end) {
+        Loads t0, t1;
+        load(t0, key0);
+        for (;;) {
+            const bool more = key0 + step < end;
+            if (more) load(t1, key0 + step);
+            compute(t0, key0);
+            if (!more) break;
+            key0 += step;
+            t0 = t1;
+        }
+    }
+
+    // the waves' parts together
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) settle(acc[d]);
+    l = sum_of_groups(l);
+    __syncthreads();
+    float* o_lds = reinterpret_cast<float*>(lds);  // [waves][16][D]
+    __shared__ float m_lds[kWaves][16], l_lds[kWaves][16];
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(o_lds + (wave * 16 + q) * D + 16 * d + 4 * g) = acc[d];
+    if (g == 0) {
+        m_lds[wave][q] = m;
+        l_lds[wave][q] = l;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = threadIdx.x; i < 16 * (D / 4); i += 64 * kWaves) {
+        const int row = i / (D / 4), d = i % (D / 4) * 4, head = 16 * gt + row;
+        if (head >= G) continue;
+        const int qh = h * G + head;
+        float most = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) most = fmaxf(most, m_lds[w][row]);
+        const bool alone = n_parts == 1;
+        const float sink = a.sinks && alone ? bf16_bits_to_f32(a.sinks[qh]) * kLog2e : -INFINITY;
+        most = fmaxf(most, sink);
+        const float base = most == -INFINITY ? 0.f : most;
+        float sum = a.sinks && alone ? __builtin_amdgcn_exp2f(sink - base) : 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(m_lds[w][row] - base);
+            sum += f * l_lds[w][row];
+            o += f * *reinterpret_cast<const f32x4*>(o_lds + (w * 16 + row) * D + d);
+        }
+        if (alone) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            *reinterpret_cast<u32x2*>(a.out + ((size_t)b * a.n_heads + qh) * D + d) = u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+        } else {
+            const size_t at = (size_t)item * a.n_heads + qh;
+            *reinterpret_cast<f32x4*>(a.part_o + at * D + d) = o;
+            if (d == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{most, sum};
+        }
+    }
+    if (part == 0 && h == 0 && gt == 0 && threadIdx.x == 0) {
+        a.plan[2 * b] = item;
+        a.plan[2 * b + 1] = n_parts;
+    }
+}
+
+// The parts of sequences that were cut, joined: a block to a sequence and some heads; a row of D floats to D / 4 lanes.
+template <int D>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionDecodeArgs a, int heads_per_block) {
+    constexpr int kLanes = D / 4, kAtOnce = 256 / kLanes;
+    const int b = blockIdx.x, first = a.plan[2 * b], n = a.plan[2 * b + 1];
+    if (n == 1) return;
+    __shared__ float sums[kAtOnce];
+    __shared__ __attribute__((aligned(16))) float rows[kAtOnce][D];
+    __shared__ float waves[4];
+    const int slot = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+    for (int head = blockIdx.y * heads_per_block; head < min(a.n_heads, (int)(blockIdx.y + 1) * heads_per_block); ++head) {
+        const float sink = a.sinks ? bf16_bits_to_f32(a.sinks[head]) * kLog2e : -INFINITY;
+        float most = sink;
+        for (int i = threadIdx.x; i < n; i += 256) most = fmaxf(most, a.part_ml[2 * ((size_t)(first + i) * a.n_heads + head)]);
+        most = fmaxf(most, __shfl_xor(most, 1));
+        most = fmaxf(most, __shfl_xor(most, 2));
+        most = fmaxf(most, __shfl_xor(most, 4));
+        most = fmaxf(most, __shfl_xor(most, 8));
+        most = max_of_groups(most);
+        __syncthreads();  // the last head's rows have been read
+        if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = most;
+        __syncthreads();
+        most = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+        const float base = most == -INFINITY ? 0.f : most;
+        float sum = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int i = slot; i < n; i += kAtOnce) {
+            const size_t at = (size_t)(first + i) * a.n_heads + head;
+            const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * at);
+            const float f = __builtin_amdgcn_exp2f(ml[0] - base);
+            sum += f * ml[1];
+            o += f * *reinterpret_cast<const f32x4*>(a.part_o + at * D + d);
+        }
+        if (d == 0) sums[slot] = sum;
+        *reinterpret_cast<f32x4*>(&rows[slot][d]) = o;
+        __syncthreads();
+        if (threadIdx.x < D / 2) {
+            float total = a.sinks ? __builtin_amdgcn_exp2f(sink - base) : 0.f, x = 0.f, y = 0.f;
+            for (int i = 0; i < kAtOnce; ++i) {
+                total += sums[i];
+                x += rows[i][2 * threadIdx.x];
+                y += rows[i][2 * threadIdx.x + 1];
+            }
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+            reinterpret_cast<uint32_t*>(a.out + ((size_t)b * a.n_heads + head) * D)[threadIdx.x] = pack_bf16x2(x * inv, y * inv);
+        }
+    }
+}
+
+// Pieces per head over all sequences: with n of them per KV head and 16 query heads there are at most n + batch.
+static int most_items(int batch, int n_kv_heads, int group_tiles, int* pieces) {
+    *pieces = std::max(1, kDecodePieces / (n_kv_heads * group_tiles));
+    return *pieces + batch;
+}
+static int group_tiles_of(int n_heads, int n_kv_heads) { return ceil_div(n_heads / n_kv_heads, 16); }
+
+size_t attention_decode_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, size_t* ml, size_t* o) {
+    int pieces;
+    const size_t items = most_items(batch, n_kv_heads, group_tiles_of(n_heads, n_kv_heads), &pieces);
+    auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    *ml = up((size_t)batch * 8);
+    *o = *ml + up(items * n_heads * 8);
+    return *o + up(items * n_heads * head_dim * 4);
+}
+
+int launch_attention_decode(AttentionDecodeArgs a, int head_dim, hipStream_t stream) {
+    const int group_tiles = group_tiles_of(a.n_heads, a.n_kv_heads);
+    const int items = most_items(a.batch, a.n_kv_heads, group_tiles, &a.pieces);
+    const dim3 grid((unsigned)(items * a.n_kv_heads * group_tiles));
+    const long long room = (long long)a.max_pages << a.page_shift;
+    const long long most = a.window ? std::min<long long>(room, (long long)a.window + kTile - 1) : room;
+    a.min_piece = most <= 256 ? 256 : 128;  // a short window is one piece: no parts to join
+    const bool join = most > a.min_piece;
+    auto run = [&](auto kernel, auto joiner) {
+        hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, stream, a);
+        int rc = launch_status();
+        if (rc || !join) return rc;
+        const int per_block = std::max(1, ceil_div(a.batch * std::min(a.n_heads, 256), 2048));
+        hipLaunchKernelGGL(joiner, dim3((unsigned)a.batch, (unsigned)ceil_div(a.n_heads, per_block)), dim3(256), 0, stream, a, per_block);
+        return launch_status();
+    };
+    const bool mx = a.k_scales != nullptr;
+    if (head_dim == 64)
+        return mx ? run(attention_decode_kernel<64, true>, attention_join_kernel<64>) : run(attention_decode_kernel<64, false>, attention_join_kernel<64>);
+    return mx ? run(attention_decode_kernel<128, true>, attention_join_kernel<128>) : run(attention_decode_kernel<128, false>, attention_join_kernel<128>);
+}
+
+}  // namespace moe

@@ -1,0 +1,246 @@
+// Causal attention over packed prompts: out = softmax(scale q K^T, sinks) V, query heads in groups that share a key/value head.
+#include <algorithm>
+
+#include "attention.h"
+#include "kernels.h"
+
+namespace moe {
+
+namespace {
+
+constexpr int kWaves = 4, kRows = 32 * kWaves, kKeys = 64;  // query rows of a block, 32 to a wave; keys that it takes at a time
+
+struct Span {
+    int begin, rows;
+};
+MOE_DEVICE Span span_of(const int* starts, int s, int total) {
+    const int begin = min(max(starts[s], 0), total);
+    return {begin, min(max(starts[s + 1], begin), total) - begin};
+}
+
+}  // namespace
+
+// Block: 128 rows of one head of one sequence; wave: 32 of them, against tiles of 64 keys that the block stages in LDS a tile ahead.  S^T = K Q^T puts a
+// query row into two lanes (l and l + 32), so that its running maximum is a lane's but for one exchange, its sum a lane's until the end, and
+// P^T the second product's operand as it stands: O^T = V^T P^T, V^T read from LDS as columns.  P is rounded to bf16 for that product (half
+// a step is up to 2^-8 of a weight, as that of the bf16 result); its sum is taken before that, in fp32.  Statistics are in powers of two.
+// Longest blocks first.  Bound by the matrix units and, with heads of 64, by the exponentials and their neighbours.
+template <int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void attention_prefill_kernel(AttentionPrefillArgs a) {
+    constexpr int kRow = 2 * D, kSteps = D / 16, kDims = D / 32, kChunks = D / 8, kLoads = kKeys * kChunks / (64 * kWaves);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5;
+
+    // heads of a group on one XCD (blocks go to them in turn), where its L2 holds their keys
+    int head, rank;
+    if (a.n_heads % 8 == 0) {
+        const int each = a.n_heads / 8, at = blockIdx.x / 8;
+        head = blockIdx.x % 8 * each + at % each;
+        rank = at / each;
+    } else {
+        head = blockIdx.x % a.n_heads;
+        rank = blockIdx.x / a.n_heads;
+    }
+    int tiles = 0;
+    auto tiles_of = [&](int s) { return ceil_div(span_of(a.q_starts, s, a.total_q).rows, kRows); };
+    for (int base = 0; base < a.n_seqs; base += 64) tiles += wave_sum(base + lane < a.n_seqs ? tiles_of(base + lane) : 0);
+    int seq, tile;
+    if (rank >= tiles || !find_item(a.n_seqs, tiles - 1 - rank, tiles_of, seq, tile)) return;
+    const Span qs = span_of(a.q_starts, seq, a.total_q), ks = span_of(a.k_starts, seq, a.total_k);
+    const int ahead = ks.rows - qs.rows;  // query i sees keys up to i + ahead
+    const int row0 = tile * kRows, kv_head = head / (a.n_heads / a.n_kv_heads);
+    const int end = min(row0 + kRows, qs.rows) + ahead;  // past the last key that the block sees
+    const int begin = a.window ? max(0, row0 + ahead - a.window + 1) & ~(kKeys - 1) : 0;
+
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][kKeys * kRow];
+
+    const int wave_row = row0 + 32 * wave, row = min(wave_row + col, qs.rows - 1);
+    const int last = row + ahead, first = a.window ? last - a.window + 1 : 0;  // what this lane's row sees
+    u32x4 qf[kSteps];
+    {
+        const uint16_t* q = a.q + (size_t)(qs.begin + row) * a.q_stride + (size_t)head * D;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) qf[s] = *reinterpret_cast<const u32x4*>(q + 16 * s + 8 * hi);
+    }
+    f32x16 acc[kDims];
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const float scale = a.scale * kLog2e;
+
+    u32x4 kr[kLoads], vr[kLoads];
+    const uint16_t* k_base = a.k + (size_t)ks.begin * a.k_stride + (size_t)kv_head * D;
+    const uint16_t* v_base = a.v + (size_t)ks.begin * a.v_stride + (size_t)kv_head * D;
+    auto load = [&](int key0) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int at = threadIdx.x + 64 * kWaves * i, r = min(key0 + at / kChunks, ks.rows - 1), c = at % kChunks;
+            kr[i] = *reinterpret_cast<const u32x4*>(k_base + (size_t)r * a.k_stride + 8 * c);
+            vr[i] = *reinterpret_cast<const u32x4*>(v_base + (size_t)r * a.v_stride + 8 * c);
+        }
+    };
+    // chunk c of row r at c ^ (r % 8) for K, which is read by rows, at c ^ 2 (r % 4) for V, read by columns of four rows
+    auto store = [&](int buffer, int key0) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int at = threadIdx.x + 64 * kWaves * i, r = at / kChunks, c = at % kChunks;
+            if (key0 + r >= ks.rows) vr[i] = u32x4{0, 0, 0, 0};  // a weight of 0 does not undo a NaN
+            *reinterpret_cast<u32x4*>(&lds[buffer][0][r * kRow + (c ^ (r & 7)) * 16]) = kr[i];
+            *reinterpret_cast<u32x4*>(&lds[buffer][1][r * kRow + (c ^ ((r & 3) << 1)) * 16]) = vr[i];
+        }
+    };
+    auto v_column = [&](const uint8_t* v, int key, int d) {  // keys key .. key + 3 (+ 4 in the upper half), the lane's dimension of 32 d ..
+        const int i = lane & 15, r = key + 4 * hi + (i >> 2), c = 4 * d + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
+        return lds_column_of_4(v + r * kRow + (c ^ ((r & 3) << 1)) * 16 + (i & 1) * 8);
+    };
+    auto compute = [&](int buffer, int key0) {
+        const uint8_t* k = lds[buffer][0];
+        const uint8_t* v = lds[buffer][1];
+        f32x16 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                const int r = 32 * t + col;
+                s[t] = mfma_32x32x16(*reinterpret_cast<const u32x4*>(k + r * kRow + ((2 * j + hi) ^ (r & 7)) * 16), qf[j], s[t]);
+            }
+        }
+        settle(s[0], s[1]);
+        const bool masked = key0 + kKeys - 1 > wave_row + ahead || (a.window && key0 < wave_row + 31 + ahead - a.window + 1);
+        if (masked) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = key0 + 32 * t + 8 * (i / 4) + 4 * hi + i % 4;
+                    if (key > last || key < first) s[t][i] = -INFINITY;
+                }
+        }
+        float most = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = fmaxf(most, s[t][i]);
+        most = fmaxf(m, max_of_halves(most) * scale);
+        if (__any(most > m)) {
+            const float down = most == m ? 1.f : __builtin_amdgcn_exp2f(m - most);
+            m = most;
+            l *= down;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) acc[d] *= down;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        u32x4 p[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[t][i], scale, -base)), y = __builtin_amdgcn_exp2f(fmaf(s[t][i + 1], scale, -base));
+                l += x + y;
+                p[2 * t + i / 8][i % 8 / 2] = pack_bf16x2(x, y);
+            }
+        bool odd = false;  // an infinity or a NaN among values that some row does not see: 0 times it is not 0
+        if (masked) {
+            uint32_t most_bits = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const u32x2 x = v_column(v, 16 * j + 8 * e, d);
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) most_bits = max(most_bits, max(x[w] & 0x7FFFu, x[w] >> 16 & 0x7FFFu));
+                    }
+            odd = __any(most_bits >= 0x7F80u);
+        }
+        auto values = [&](int j, int d) {
+            const u32x2 x = v_column(v, 16 * j, d), y = v_column(v, 16 * j + 8, d);
+            return u32x4{x[0], x[1], y[0], y[1]};
+        };
+        if (!odd) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int d = 0; d < kDims; ++d) acc[d] = mfma_32x32x16(values(j, d), p[j], acc[d]);
+        } else {  // the finite ones as ever, then the others a key at a time, added where the key is seen
+            auto odd_ones = [](uint32_t x) { return ((x & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u); };
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int d = 0; d < kDims; ++d) {
+                    const u32x4 x = values(j, d);
+                    u32x4 left;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) left[w] = x[w] & ~odd_ones(x[w]);
+                    acc[d] = mfma_32x32x16(left, p[j], acc[d]);
+                    settle(acc[d]);
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = key0 + 16 * j + i, e = (i >> 3) * 4 + (i & 3);  // element e of the half (i >> 2) & 1
+                        const bool mine = ((i >> 2) & 1) == hi, seen = key <= last && key >= first;
+                        u32x4 one;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) one[w] = x[w] & odd_ones(x[w]) & (mine && (e >> 1) == w ? ((e & 1) ? 0xFFFF0000u : 0xFFFFu) : 0u);
+                        f32x16 o;
+#pragma unroll
+                        for (int n = 0; n < 16; ++n) o[n] = 0.f;
+                        o = mfma_32x32x16(one, p[j], o);
+                        settle(o);
+#pragma unroll
+                        for (int n = 0; n < 16; ++n) acc[d][n] = seen ? acc[d][n] + o[n] : acc[d][n];
+                    }
+                }
+        }
+    };
+
+    if (begin < end) {
+        load(begin);
+        store(0, begin);
+        __syncthreads();
+        int buffer = 0;
+        for (int key0 = begin; key0 < end; key0 += kKeys) {
+            const bool more = key0 + kKeys < end;
+            if (more) load(key0 + kKeys);
+            // whether any row of the wave sees any of these keys
+            if (key0 <= wave_row + 31 + ahead && (!a.window || key0 + kKeys > wave_row + ahead - a.window + 1) && wave_row < qs.rows) compute(buffer, key0);
+            if (more) store(buffer ^ 1, key0 + kKeys);
+            __syncthreads();
+            buffer ^= 1;
+        }
+    }
+
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) settle(acc[d]);
+    if (a.sinks) {
+        const float sink = bf16_bits_to_f32(a.sinks[head]) * kLog2e, most = fmaxf(m, sink), base = most == -INFINITY ? 0.f : most;
+        const float down = __builtin_amdgcn_exp2f(m - base);
+        l = sum_of_halves(l) * down + __builtin_amdgcn_exp2f(sink - base);
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) acc[d] *= down;
+    } else {
+        l = sum_of_halves(l);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (wave_row + col < qs.rows) {
+        uint16_t* out = a.out + (size_t)(qs.begin + row) * a.out_stride + (size_t)head * D;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<u32x2*>(out + 32 * d + 2 * i + 4 * hi) =
+                    u32x2{pack_bf16x2(acc[d][i] * inv, acc[d][i + 1] * inv), pack_bf16x2(acc[d][i + 2] * inv, acc[d][i + 3] * inv)};
+    }
+}
+
+int launch_attention_prefill(const AttentionPrefillArgs& a, int head_dim, hipStream_t stream) {
+    const long long blocks = ((long long)a.total_q / kRows + std::min(a.n_seqs, a.total_q)) * a.n_heads;  // as many as there can be
+    if (blocks > 0x7FFFFFFFll / (64 * kWaves)) return MOE_ERR_LIMIT;
+    if (head_dim == 64) hipLaunchKernelGGL(attention_prefill_kernel<64>, dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream, a);
+    else hipLaunchKernelGGL(attention_prefill_kernel<128>, dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream, a);
+    return launch_status();
+}
+
+}  // namespace moe

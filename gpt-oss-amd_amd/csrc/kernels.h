@@ -211,6 +211,78 @@ void int4_tiled_bytes(int rows, int K, int group, size_t* codes, size_t* scales,
 int launch_int4_repack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int rows, int K, int group, uint8_t* tiled_codes,
                        uint16_t* tiled_scales, uint8_t* tiled_zeros, hipStream_t stream);
 
+// ---- rope_kv.hip -------------------------------------------------------------------------------
+struct RopeKvArgs {
+    const void* rows;       // [n_tokens, stride]: heads' queries, keys, values; fp32 or bf16
+    long long stride;       // elements
+    const int* positions;
+    const float* inv_freq;  // [rotary_dim / 2]
+    uint16_t* q;            // or nullptr, as the next two
+    uint16_t* k;
+    uint16_t* v;
+    uint8_t* cache_k;       // [n_pages, n_kv_heads, page_size, head_dim] bf16, or e4m3 with scales; or nullptr
+    uint8_t* cache_v;
+    uint8_t* k_scales;
+    uint8_t* v_scales;
+    const int* slots;
+    int n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, page_shift;
+    long long n_slots;
+    float scale;
+};
+int launch_rope_kv_write(const RopeKvArgs& a, bool bf16_rows, hipStream_t stream);
+
+// ---- attention_decode.hip ----------------------------------------------------------------------
+constexpr int kDecodePieces = 1024;  // blocks that a launch aims at: four to a compute unit
+struct AttentionDecodeArgs {
+    uint16_t* out;
+    const uint16_t* q;
+    const void* k;            // cache
+    const void* v;
+    const uint8_t* k_scales;  // or nullptr: bf16
+    const uint8_t* v_scales;
+    const int* page_table;    // [batch, max_pages]
+    const int* lengths;
+    const uint16_t* sinks;    // or nullptr
+    int* plan;                // workspace: [batch, 2] first part, parts
+    float* part_ml;           // [parts, n_heads, 2]
+    float* part_o;            // [parts, n_heads, head_dim]
+    int batch, n_heads, n_kv_heads, max_pages, n_pages, page_shift, window;
+    float scale;
+    int pieces, min_piece;    // set by the launcher
+};
+size_t attention_decode_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, size_t* ml, size_t* o);
+int launch_attention_decode(AttentionDecodeArgs a, int head_dim, hipStream_t stream);
+
+// ---- attention_prefill.hip ---------------------------------------------------------------------
+struct AttentionPrefillArgs {
+    uint16_t* out;
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    const int* q_starts;    // [n_seqs + 1]
+    const int* k_starts;
+    const uint16_t* sinks;  // or nullptr
+    long long out_stride, q_stride, k_stride, v_stride;  // elements from token to token
+    int n_seqs, total_q, total_k, n_heads, n_kv_heads, window;
+    float scale;
+};
+int launch_attention_prefill(const AttentionPrefillArgs& a, int head_dim, hipStream_t stream);
+
+// ---- logprobs.hip ------------------------------------------------------------------------------
+struct LogprobArgs {
+    const void* logits;
+    long long stride;
+    const int* tokens;
+    float* logprobs;      // or nullptr, as the next three
+    float* entropy;
+    float* top_logprobs;
+    int* top_indices;
+    void* workspace;
+    int n_tokens, vocab, top_k;
+};
+size_t logprob_workspace(int n_tokens, int vocab, int top_k);
+int launch_token_logprobs(const LogprobArgs& a, bool bf16_logits, hipStream_t stream);
+
 // ---- mxfp4.hip ---------------------------------------------------------------------------------
 void mxfp4_tiled_bytes(int rows, int K, size_t* block_bytes, size_t* scale_bytes);
 int launch_fill_zero(uint32_t* words, size_t n, hipStream_t stream);

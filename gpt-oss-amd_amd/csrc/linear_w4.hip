@@ -4,6 +4,7 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "mx8.h"
 
 namespace moe {
 
@@ -15,16 +16,6 @@ constexpr int kUnit = 256;  // contraction elements of a wave: two chunks of 128
 constexpr int max_waves(int group, int nt) {
     if (nt == 1) return 16;
     return group == 32 ? 8 : group == 64 ? 12 : 16;
-}
-
-// e4m3 values times a power of two (its exponent counts: the bits of 0 are 2^-127), to bf16: exact, with three mantissa bits, but for denormals.
-MOE_DEVICE u32x4 e4m3x8_to_bf16(uint32_t lo, uint32_t hi, float scale) {
-    u32x4 v;
-    v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
-    v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
-    v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
-    v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
-    return v;
 }
 
 // Floats of the LDS that a wave keeps its partial tiles in, those of two steps; a chunk of 16 rows of x goes through it while it is loaded.

@@ -323,6 +323,89 @@ MOE_API int moe_int4_repack(const uint8_t* codes, const moe_bf16_t* scales, cons
                             uint8_t* tiled_codes, moe_bf16_t* tiled_scales, uint8_t* tiled_zeros, moe_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Attention and what surrounds it (the reference's own are kernels of its forward pass for one cache layout:
+ * src/hip/split_qkv.hip, rope.hip, attention.hip; these are operators of their own for a paged cache)
+ * ---------------------------------------------------------------------------------------- */
+
+enum { MOE_ROWS_F32 = 0, MOE_ROWS_BF16 = 1 };  /* type of an operator's rows */
+
+/* A paged key-value cache: n_pages pages of page_size token slots; slot s of the cache is slot s % page_size of page s / page_size.
+ * k, v [n_pages, n_kv_heads, page_size, head_dim]: bf16 (scales NULL), or e4m3 codes with k_scales, v_scales [n_pages, n_kv_heads, page_size,
+ * head_dim / 32] e8m0 as moe_rope_kv_write writes them: byte b is 2^(b - 127), 255 a NaN; values that bf16 holds (2^-126 to 2^128).
+ * page_size a power of two from 16 to 2^20, head_dim 64 or 128, n_kv_heads <= 1024, n_pages * page_size < 2^31; k and v 16-byte
+ * aligned.  The struct is host memory, read during the call. */
+typedef struct moe_kv_cache {
+    uint32_t struct_bytes;   /* sizeof(moe_kv_cache) of the caller's header */
+    int32_t n_pages;
+    int32_t page_size;
+    int32_t n_kv_heads;
+    int32_t head_dim;
+    void* k;
+    void* v;
+    uint8_t* k_scales;       /* both or neither */
+    uint8_t* v_scales;
+} moe_kv_cache;
+
+/* Rotary embedding and cache write.  qkv holds n_tokens rows, `stride` elements apart, of n_heads queries, n_kv_heads keys and n_kv_heads values of
+ * head_dim each, fp32 or bf16 (qkv_type MOE_ROWS_*).  Of every query and key the first rotary_dim values turn: with p = positions[token],
+ * i < rotary_dim / 2, a = p * inv_freq[i] (exact, in fp64), u = x[i], v = x[i + rotary_dim / 2]:
+ *   x[i] = scale (u cos a - v sin a),  x[i + rotary_dim / 2] = scale (v cos a + u sin a)   in fp32, cos and sin to 2^-22
+ * Then what is asked for, at least one:
+ *   q, k, v   [n_tokens, n_heads or n_kv_heads, head_dim] bf16, each or NULL (k and v for moe_attention_prefill)
+ *   cache     keys and values of token t to slot slots[t], or nowhere if that is not in [0, n_pages * page_size); no other slot changes.  The slots of a
+ *             call have to differ.  In 8 bits: per 32 values the smallest power of two, from 2^-126, that leaves the largest at 448 or below,
+ *             codes rounded to nearest even from fp32; a group with an infinity or a NaN has a NaN for its scale and for every code
+ * cache and slots both or neither.  rotary_dim <= head_dim, a multiple of 8 (of 64 with an 8-bit cache), 0 for none (inv_freq may be NULL);
+ * n_heads <= 1024; stride >= (n_heads + 2 n_kv_heads) head_dim and a multiple of 4; n_tokens < 2^31 - 255; qkv, q, k, v 16-byte aligned, the
+ * rest 4-byte.  No output may overlap an input. */
+MOE_API int moe_rope_kv_write(const void* qkv, int qkv_type, long long stride, const int* positions, const float* inv_freq, int n_tokens, int n_heads,
+                              int n_kv_heads, int head_dim, int rotary_dim, float scale, moe_bf16_t* q, moe_bf16_t* k, moe_bf16_t* v,
+                              const moe_kv_cache* cache, const int* slots, moe_stream_t stream);
+
+/* Attention of one query row a sequence over the cache.  Sequence b has lengths[b] keys (below 0 none; no more than max_pages * page_size), key j in slot
+ * j % page_size of page page_table[b, j / page_size]; its query, the last of them, sees the keys j >= lengths[b] - window (all with window 0).
+ * Query heads g, g + 1, .. share a key/value head: head h reads key/value head h / (n_heads / n_kv_heads).
+ *   s[j] = scale q . k[j],  out = sum_j exp(s[j]) v[j] / (sum_j exp(s[j]) + exp(sinks[h]))    (without sinks: without their term)
+ * A query that sees nothing has zeros.  Products of bf16 values, sums and statistics in fp32, weights rounded to bf16; the result is rounded once.
+ * A page number outside [0, n_pages) is a page without keys, and page numbers behind a sequence's last key are not looked at: a table may hold
+ * anything there, as may the slots.  Deterministic, but the sum over keys is cut into pieces that depend on all the lengths of a call.
+ * q, out [batch, n_heads, head_dim] bf16, page_table [batch, max_pages], lengths [batch], sinks [n_heads] bf16 or NULL.  n_heads <= 1024, a multiple of
+ * n_kv_heads; scale > 0 and finite; batch <= 65535; max_pages * page_size <= 2^30; q and out 16-byte aligned.  workspace:
+ * moe_attention_decode_workspace_bytes (0 for sizes that the call rejects; a batch's serves smaller ones), 16-byte aligned; its content
+ * does not matter.  Calls that overlap in time need workspaces of their own.  out may not overlap an input. */
+MOE_API size_t moe_attention_decode_workspace_bytes(int batch, int n_heads, int n_kv_heads, int head_dim);
+MOE_API int moe_attention_decode(moe_bf16_t* out, const moe_bf16_t* q, const moe_kv_cache* cache, const int* page_table, const int* lengths, int batch,
+                                 int n_heads, int max_pages, int window, float scale, const moe_bf16_t* sinks, void* workspace, size_t workspace_bytes,
+                                 moe_stream_t stream);
+
+/* Causal attention over prompts packed one after another: sequence s has the query rows q_starts[s] .. q_starts[s + 1] - 1 of total_q and the key and value
+ * rows k_starts[s] .. k_starts[s + 1] - 1 of total_k.  Its queries are its last positions: query i of n sees key j of m if j <= i + m - n and, with
+ * a window, j > i + m - n - window.  The rest as moe_attention_decode.  Rows that belong to no sequence are not written.  What one row
+ * sees does not depend on keys that it does not see, whatever these and their values hold; a row's result does not depend on other sequences.
+ * q, out [total_q, n_heads, head_dim], k, v [total_k, n_kv_heads, head_dim] bf16, *_stride elements from token to token (at least a token's, a
+ * multiple of 8); starts ascending (what lies outside the rows is cut off).  head_dim 64 or 128; n_seqs <= 65535; total_q * n_heads < 2^30; all
+ * tensors 16-byte aligned, starts 4-byte. */
+MOE_API int moe_attention_prefill(moe_bf16_t* out, const moe_bf16_t* q, const moe_bf16_t* k, const moe_bf16_t* v, const int* q_starts,
+                                  const int* k_starts, int n_seqs, int total_q, int total_k, int n_heads, int n_kv_heads, int head_dim,
+                                  long long out_stride, long long q_stride, long long k_stride, long long v_stride, int window, float scale,
+                                  const moe_bf16_t* sinks, moe_stream_t stream);
+
+/* Log probabilities from rows of logits [n_tokens, vocab], `stride` elements apart, fp32 or bf16 (logits_type MOE_ROWS_*); with p = softmax(l):
+ *   logprobs[t]      log p[tokens[t]]; NaN for a token outside [0, vocab)
+ *   entropy[t]       -sum p log p
+ *   top_indices[t]   the top_k largest logits in descending order, equal ones: the lower index; top_logprobs[t] their log p
+ * each or NULL, at least one (the two of top_k both or neither, top_k 0 without).  Logits of -infinity have no weight.  A row with a NaN or a
+ * +infinity, or with nothing but -infinity, has NaN for all its values; its indices are distinct and in range.  Sums in fp32, apart from the
+ * largest logit's own weight, so that small entropies and log probabilities next to 0 keep their precision.
+ * top_k <= 32 and <= vocab; vocab <= 2^30; stride >= vocab; logits aligned to their type, the rest 4-byte.  workspace:
+ * moe_token_logprobs_workspace_bytes (that of more rows serves fewer; NULL where it is 0), 16-byte aligned; its content does not matter, and calls that
+ * overlap in time need their own. */
+MOE_API size_t moe_token_logprobs_workspace_bytes(int n_tokens, int vocab, int top_k);
+MOE_API int moe_token_logprobs(const void* logits, int logits_type, long long stride, const int* tokens, int n_tokens, int vocab, int top_k,
+                               float* logprobs, float* entropy, float* top_logprobs, int* top_indices, void* workspace, size_t workspace_bytes,
+                               moe_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * MXFP4 (no counterpart at run time in the reference, which dequantises offline:
  * tools/model_export/gpt-oss-20b/export_model_bin.py:95-133)
  * ---------------------------------------------------------------------------------------- */
