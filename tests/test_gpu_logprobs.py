@@ -110,6 +110,8 @@ def test_rows_without_probabilities_and_tokens_out_of_range(pkg, dev):
         for t in range(7):
             i = index[t].tolist()
             assert len(set(i)) == 32 and min(i) >= 0 and max(i) < V, (t, i)
+        l[6, : V - 20], l[6, 5] = -inf, float("nan")  # a NaN among values without weight
+        assert torch.isnan(call(pkg, l, tokens, 7)[1][6])
         tokens[6] = -1
         assert torch.isnan(call(pkg, l, tokens, 0)[0][6])
 
