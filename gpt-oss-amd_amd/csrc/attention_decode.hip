@@ -55,7 +55,8 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(Attention
     double total = 0.0;  // keys of all sequences, exact
     for (int base = 0; base < a.batch; base += 64) total += wave_sum(base + lane < a.batch ? (double)seen_of(a, base + lane).keys() : 0.0);
     const long long even = (long long)(total / a.pieces) + 1;
-    const int piece = (int)min(max((even + kTile - 1) / kTile * kTile, (long long)a.min_piece), 1ll << 30);
+    constexpr int kStep = kWaves * kTile;
+    const int piece = (int)min(max((even + kStep - 1) / kStep * kStep, (long long)a.min_piece), 1ll << 30);
     int b, part;
     auto pieces_of = [&](int s) { return max(1, ceil_div(seen_of(a, s).keys(), piece)); };
     if (!find_item(a.batch, item, pieces_of, b, part)) return;
@@ -111,8 +112,8 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(Attention
 #pragma unroll
         for (int i = 0; i < Loads::kLoads; ++i) {
             const int half = i * Loads::kRows / 16, at = i * Loads::kRows % 16 + r;
-            t.k[i] = *reinterpret_cast<const u32x4*>(kp[half] + at * Loads::kRowBytes + 16 * c);
-            t.v[i] = *reinterpret_cast<const u32x4*>(vp[half] + at * Loads::kRowBytes + 16 * c);
+            t.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp[half] + at * Loads::kRowBytes + 16 * c));
+            t.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vp[half] + at * Loads::kRowBytes + 16 * c));
             if constexpr (MX) {
                 t.ks[i] = ksp[half][at * (D / 32) + c / 2];
                 t.vs[i] = vsp[half][at * (D / 32) + c / 2];
@@ -201,18 +202,20 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(Attention
         lds_in_order();
     };
 
-    const int step = kWaves * kTile;
     int key0 = begin + wave * kTile;
     if (key0 < end) {
         Loads t0, t1;
         load(t0, key0);
+        if (key0 + kStep < end) load(t1, key0 + kStep);
         for (;;) {
-            const bool more = key0 + step < end;
-            if (more) load(t1, key0 + step);
             compute(t0, key0);
-            if (!more) break;
-            key0 += step;
-            t0 = t1;
+            if (key0 + 2 * kStep < end) load(t0, key0 + 2 * kStep);
+            key0 += kStep;
+            if (key0 >= end) break;
+            compute(t1, key0);
+            if (key0 + 2 * kStep < end) load(t1, key0 + 2 * kStep);
+            key0 += kStep;
+            if (key0 >= end) break;
         }
     }
 
@@ -265,49 +268,47 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(Attention
     }
 }
 
-// The parts of sequences that were cut, joined: a block to a sequence and some heads; a row of D floats to D / 4 lanes.
+// The parts of sequences that were cut, joined: a block to a sequence and some heads; a row of D floats to D / 4 lanes, which take every kAtOnce-th part with
+// a maximum of their own, so that no load waits for another's value but for the plan.
 template <int D>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionDecodeArgs a, int heads_per_block) {
     constexpr int kLanes = D / 4, kAtOnce = 256 / kLanes;
     const int b = blockIdx.x, first = a.plan[2 * b], n = a.plan[2 * b + 1];
     if (n == 1) return;
-    __shared__ float sums[kAtOnce];
+    __shared__ f32x2 stats[kAtOnce];
     __shared__ __attribute__((aligned(16))) float rows[kAtOnce][D];
-    __shared__ float waves[4];
     const int slot = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
     for (int head = blockIdx.y * heads_per_block; head < min(a.n_heads, (int)(blockIdx.y + 1) * heads_per_block); ++head) {
-        const float sink = a.sinks ? bf16_bits_to_f32(a.sinks[head]) * kLog2e : -INFINITY;
-        float most = sink;
-        for (int i = threadIdx.x; i < n; i += 256) most = fmaxf(most, a.part_ml[2 * ((size_t)(first + i) * a.n_heads + head)]);
-        most = fmaxf(most, __shfl_xor(most, 1));
-        most = fmaxf(most, __shfl_xor(most, 2));
-        most = fmaxf(most, __shfl_xor(most, 4));
-        most = fmaxf(most, __shfl_xor(most, 8));
-        most = max_of_groups(most);
-        __syncthreads();  // the last head's rows have been read
-        if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = most;
-        __syncthreads();
-        most = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
-        const float base = most == -INFINITY ? 0.f : most;
-        float sum = 0.f;
+        float most = -INFINITY, sum = 0.f;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int i = slot; i < n; i += kAtOnce) {
             const size_t at = (size_t)(first + i) * a.n_heads + head;
             const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * at);
-            const float f = __builtin_amdgcn_exp2f(ml[0] - base);
-            sum += f * ml[1];
-            o += f * *reinterpret_cast<const f32x4*>(a.part_o + at * D + d);
+            const f32x4 row = *reinterpret_cast<const f32x4*>(a.part_o + at * D + d);
+            const float now = fmaxf(most, ml[0]), base = now == -INFINITY ? 0.f : now;
+            const float f = __builtin_amdgcn_exp2f(most - base), g = __builtin_amdgcn_exp2f(ml[0] - base);
+            most = now;
+            sum = sum * f + ml[1] * g;
+            o = o * f + row * g;
         }
-        if (d == 0) sums[slot] = sum;
+        const float sink = a.sinks ? bf16_bits_to_f32(a.sinks[head]) * kLog2e : -INFINITY;
+        __syncthreads();  // the last head's rows have been read
+        if (d == 0) stats[slot] = f32x2{most, sum};
         *reinterpret_cast<f32x4*>(&rows[slot][d]) = o;
         __syncthreads();
         if (threadIdx.x < D / 2) {
+            most = sink;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) most = fmaxf(most, stats[i][0]);
+            const float base = most == -INFINITY ? 0.f : most;
             float total = a.sinks ? __builtin_amdgcn_exp2f(sink - base) : 0.f, x = 0.f, y = 0.f;
+#pragma unroll
             for (int i = 0; i < kAtOnce; ++i) {
-                total += sums[i];
-                x += rows[i][2 * threadIdx.x];
-                y += rows[i][2 * threadIdx.x + 1];
+                const float f = __builtin_amdgcn_exp2f(stats[i][0] - base);
+                total += f * stats[i][1];
+                x += f * rows[i][2 * threadIdx.x];
+                y += f * rows[i][2 * threadIdx.x + 1];
             }
             const float inv = total == 0.f ? 0.f : 1.f / total;
             reinterpret_cast<uint32_t*>(a.out + ((size_t)b * a.n_heads + head) * D)[threadIdx.x] = pack_bf16x2(x * inv, y * inv);

@@ -232,7 +232,7 @@ struct RopeKvArgs {
 int launch_rope_kv_write(const RopeKvArgs& a, bool bf16_rows, hipStream_t stream);
 
 // ---- attention_decode.hip ----------------------------------------------------------------------
-constexpr int kDecodePieces = 1024;  // blocks that a launch aims at: four to a compute unit
+constexpr int kDecodePieces = 768;  // blocks that a launch aims at: three to a compute unit, which are resident at once
 struct AttentionDecodeArgs {
     uint16_t* out;
     const uint16_t* q;
