@@ -10,6 +10,10 @@ namespace {
 
 constexpr int kWaves = 4, kRows = 32 * kWaves, kKeys = 64;  // query rows of a block, 32 to a wave; keys that it takes at a time
 
+// Half a row's weights of a tile, relative to the maximum that it knows, may add up to this before it looks for a new maximum: no tile but the first few
+// has to look for one, and with weights up to 2^10 sums stay as far from overflow as values of 2^118 allow.
+constexpr float kMostWeight = 1024.f;
+
 struct Span {
     int begin, rows;
 };
@@ -26,7 +30,7 @@ MOE_DEVICE Span span_of(const int* starts, int s, int total) {
 // a step is up to 2^-8 of a weight, as that of the bf16 result); its sum is taken before that, in fp32.  Statistics are in powers of two.
 // Longest blocks first.  Bound by the matrix units and, with heads of 64, by the exponentials and their neighbours.
 template <int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void attention_prefill_kernel(AttentionPrefillArgs a) {
+__global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefill_kernel(AttentionPrefillArgs a) {
     constexpr int kRow = 2 * D, kSteps = D / 16, kDims = D / 32, kChunks = D / 8, kLoads = kKeys * kChunks / (64 * kWaves);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5;
 
@@ -52,6 +56,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_prefill_kernel(Atten
     const int begin = a.window ? max(0, row0 + ahead - a.window + 1) & ~(kKeys - 1) : 0;
 
     __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][kKeys * kRow];
+    __shared__ int odd[2];  // the first key of the last tile in that buffer whose values were not all finite
 
     const int wave_row = row0 + 32 * wave, row = min(wave_row + col, qs.rows - 1);
     const int last = row + ahead, first = a.window ? last - a.window + 1 : 0;  // what this lane's row sees
@@ -80,12 +85,30 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_prefill_kernel(Atten
             vr[i] = *reinterpret_cast<const u32x4*>(v_base + (size_t)r * a.v_stride + 8 * c);
         }
     };
+    // Whether some row of the block does not see all of these keys.  Their values go to LDS without infinities and NaNs, which a weight of 0 does not undo;
+    // the rows that do see those get them afterwards.
+    auto cut = [&](int key0) { return key0 + kKeys - 1 > row0 + ahead || (a.window && key0 < end - a.window); };
     // chunk c of row r at c ^ (r % 8) for K, which is read by rows, at c ^ 2 (r % 4) for V, read by columns of four rows
     auto store = [&](int buffer, int key0) {
+        if (cut(key0)) {
+            auto not_finite = [](uint32_t x) { return ((x & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u); };
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const bool outside = key0 + (int)(threadIdx.x + 64 * kWaves * i) / kChunks >= ks.rows;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    if (outside) vr[i][w] = 0;
+                    const uint32_t off = not_finite(vr[i][w]);
+                    vr[i][w] &= ~off;
+                    any |= off;
+                }
+            }
+            if (any) odd[buffer] = key0;
+        }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int at = threadIdx.x + 64 * kWaves * i, r = at / kChunks, c = at % kChunks;
-            if (key0 + r >= ks.rows) vr[i] = u32x4{0, 0, 0, 0};  // a weight of 0 does not undo a NaN
             *reinterpret_cast<u32x4*>(&lds[buffer][0][r * kRow + (c ^ (r & 7)) * 16]) = kr[i];
             *reinterpret_cast<u32x4*>(&lds[buffer][1][r * kRow + (c ^ ((r & 3) << 1)) * 16]) = vr[i];
         }
@@ -109,8 +132,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_prefill_kernel(Atten
             }
         }
         settle(s[0], s[1]);
-        const bool masked = key0 + kKeys - 1 > wave_row + ahead || (a.window && key0 < wave_row + 31 + ahead - a.window + 1);
-        if (masked) {
+        if (key0 + kKeys - 1 > wave_row + ahead || (a.window && key0 < wave_row + 31 + ahead - a.window + 1)) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -119,85 +141,72 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_prefill_kernel(Atten
                     if (key > last || key < first) s[t][i] = -INFINITY;
                 }
         }
-        float most = -INFINITY;
+        u32x4 p[4];
+        auto weigh = [&](float base) {
+            float sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) most = fmaxf(most, s[t][i]);
-        most = fmaxf(m, max_of_halves(most) * scale);
-        if (__any(most > m)) {
+                for (int i = 0; i < 16; i += 2) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[t][i], scale, -base)), y = __builtin_amdgcn_exp2f(fmaf(s[t][i + 1], scale, -base));
+                    sum[0] += x;
+                    sum[1] += y;
+                    p[2 * t + i / 8][i % 8 / 2] = pack_bf16x2(x, y);
+                }
+            return sum[0] + sum[1];
+        };
+        float sum = weigh(m);
+        if (__any(!(sum < kMostWeight))) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, s[t][i]);
+            most = max_of_halves(sum < kMostWeight ? 0.f : 1.f) > 0.f ? fmaxf(m, max_of_halves(most) * scale) : m;  // of the rows that have to
             const float down = most == m ? 1.f : __builtin_amdgcn_exp2f(m - most);
             m = most;
             l *= down;
 #pragma unroll
             for (int d = 0; d < kDims; ++d) acc[d] *= down;
+            sum = weigh(m == -INFINITY ? 0.f : m);
         }
-        const float base = m == -INFINITY ? 0.f : m;
-        u32x4 p[4];
+        l += sum;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[t][i], scale, -base)), y = __builtin_amdgcn_exp2f(fmaf(s[t][i + 1], scale, -base));
-                l += x + y;
-                p[2 * t + i / 8][i % 8 / 2] = pack_bf16x2(x, y);
+            for (int d = 0; d < kDims; ++d) {
+                const u32x2 x = v_column(v, 16 * j, d), y = v_column(v, 16 * j + 8, d);
+                acc[d] = mfma_32x32x16(u32x4{x[0], x[1], y[0], y[1]}, p[j], acc[d]);
             }
-        bool odd = false;  // an infinity or a NaN among values that some row does not see: 0 times it is not 0
-        if (masked) {
-            uint32_t most_bits = 0;
+        if (cut(key0) && odd[buffer] == key0) {  // what was left out, a key at a time, added where it is seen
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int d = 0; d < kDims; ++d)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const u32x2 x = v_column(v, 16 * j + 8 * e, d);
-#pragma unroll
-                        for (int w = 0; w < 2; ++w) most_bits = max(most_bits, max(x[w] & 0x7FFFu, x[w] >> 16 & 0x7FFFu));
-                    }
-            odd = __any(most_bits >= 0x7F80u);
-        }
-        auto values = [&](int j, int d) {
-            const u32x2 x = v_column(v, 16 * j, d), y = v_column(v, 16 * j + 8, d);
-            return u32x4{x[0], x[1], y[0], y[1]};
-        };
-        if (!odd) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int d = 0; d < kDims; ++d) acc[d] = mfma_32x32x16(values(j, d), p[j], acc[d]);
-        } else {  // the finite ones as ever, then the others a key at a time, added where the key is seen
-            auto odd_ones = [](uint32_t x) { return ((x & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u); };
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int d = 0; d < kDims; ++d) settle(acc[d]);
+            for (int i = 0; i < kKeys && key0 + i < ks.rows; ++i) {
+                const int j = i >> 4, e = ((i >> 3) & 1) * 4 + (i & 3);  // element e of the half (i >> 2) & 1
+                const bool mine = ((i >> 2) & 1) == hi, seen = key0 + i <= last && key0 + i >= first;
+                const u32x4 weights = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
 #pragma unroll
                 for (int d = 0; d < kDims; ++d) {
-                    const u32x4 x = values(j, d);
-                    u32x4 left;
+                    const uint32_t x = v_base[(size_t)(key0 + i) * a.v_stride + 32 * d + col], left = mine && (x & 0x7F80u) == 0x7F80u ? x << (e & 1) * 16 : 0u;
+                    u32x4 one;
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) left[w] = x[w] & ~odd_ones(x[w]);
-                    acc[d] = mfma_32x32x16(left, p[j], acc[d]);
-                    settle(acc[d]);
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = key0 + 16 * j + i, e = (i >> 3) * 4 + (i & 3);  // element e of the half (i >> 2) & 1
-                        const bool mine = ((i >> 2) & 1) == hi, seen = key <= last && key >= first;
-                        u32x4 one;
+                    for (int w = 0; w < 4; ++w) one[w] = e >> 1 == w ? left : 0u;
+                    f32x16 o;
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) one[w] = x[w] & odd_ones(x[w]) & (mine && (e >> 1) == w ? ((e & 1) ? 0xFFFF0000u : 0xFFFFu) : 0u);
-                        f32x16 o;
+                    for (int n = 0; n < 16; ++n) o[n] = 0.f;
+                    o = mfma_32x32x16(one, weights, o);
+                    settle(o);
 #pragma unroll
-                        for (int n = 0; n < 16; ++n) o[n] = 0.f;
-                        o = mfma_32x32x16(one, p[j], o);
-                        settle(o);
-#pragma unroll
-                        for (int n = 0; n < 16; ++n) acc[d][n] = seen ? acc[d][n] + o[n] : acc[d][n];
-                    }
+                    for (int n = 0; n < 16; ++n) acc[d][n] = seen ? acc[d][n] + o[n] : acc[d][n];
                 }
+            }
         }
     };
 
     if (begin < end) {
+        if (threadIdx.x < 2) odd[threadIdx.x] = -1;
         load(begin);
+        __syncthreads();
         store(0, begin);
         __syncthreads();
         int buffer = 0;
