@@ -32,6 +32,17 @@ MOE_DEVICE u32x2 lds_column_of_4(const void* p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p)));
 }
 
+// Where 16-byte chunk c of row r of a tile of keys or values (2 D bytes a row) lies within its row in LDS: an exclusive or that gives 8 and 16 rows which are
+// read side by side, the same chunk of each, banks of their own (keys), and two or four neighbouring chunks of 4 rows (values, read by columns).
+template <int D>
+MOE_DEVICE int k_chunk(int r, int c) {
+    return c ^ (D == 64 ? (r & 7) ^ ((r >> 3) & 1) : r & 15);
+}
+template <int D>
+MOE_DEVICE int v_chunk(int r, int c) {
+    return c ^ (D == 64 ? (r & 3) << 1 : (r & 3) << 2 | (r & 2));
+}
+
 // Maximum or sum over the lanes that differ in bits 4 and 5 only (the four groups of 16), in all of them.
 MOE_DEVICE float max_of_groups(float v) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);

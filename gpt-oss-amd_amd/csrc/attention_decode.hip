@@ -130,7 +130,6 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(Attention
     auto compute = [&](Loads& t, int key0) {
         const bool whole = key0 >= seen.first && key0 + kTile <= end && t.valid[0] && t.valid[1];
         auto visible = [&](int key) { return key >= seen.first && key < end && t.valid[(key - key0) >> 4]; };
-        // to LDS: 16-byte chunk c of row r at c ^ (r % 8) for K, which is read by rows, at c ^ 2 (r % 4) for V, read by columns of four rows
         const int r0 = lane / Loads::kLanes, c = lane % Loads::kLanes;
 #pragma unroll
         for (int i = 0; i < Loads::kLoads; ++i) {
@@ -138,16 +137,15 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(Attention
             if (!whole && !visible(key0 + r)) t.v[i] = u32x4{0, 0, 0, 0};  // a weight of 0 does not undo a NaN
             uint8_t* kr = k_lds + r * kRow;
             uint8_t* vr = v_lds + r * kRow;
-            const int ks = r & 7, vs = (r & 3) << 1;
             if constexpr (MX) {
                 const float k_scale = mx_scale(t.ks[i]), v_scale = !whole && !visible(key0 + r) ? 1.f : mx_scale(t.vs[i]);
-                *reinterpret_cast<u32x4*>(kr + ((2 * c) ^ ks) * 16) = e4m3x8_to_bf16(t.k[i][0], t.k[i][1], k_scale);
-                *reinterpret_cast<u32x4*>(kr + ((2 * c + 1) ^ ks) * 16) = e4m3x8_to_bf16(t.k[i][2], t.k[i][3], k_scale);
-                *reinterpret_cast<u32x4*>(vr + ((2 * c) ^ vs) * 16) = e4m3x8_to_bf16(t.v[i][0], t.v[i][1], v_scale);
-                *reinterpret_cast<u32x4*>(vr + ((2 * c + 1) ^ vs) * 16) = e4m3x8_to_bf16(t.v[i][2], t.v[i][3], v_scale);
+                *reinterpret_cast<u32x4*>(kr + k_chunk<D>(r, 2 * c) * 16) = e4m3x8_to_bf16(t.k[i][0], t.k[i][1], k_scale);
+                *reinterpret_cast<u32x4*>(kr + k_chunk<D>(r, 2 * c + 1) * 16) = e4m3x8_to_bf16(t.k[i][2], t.k[i][3], k_scale);
+                *reinterpret_cast<u32x4*>(vr + v_chunk<D>(r, 2 * c) * 16) = e4m3x8_to_bf16(t.v[i][0], t.v[i][1], v_scale);
+                *reinterpret_cast<u32x4*>(vr + v_chunk<D>(r, 2 * c + 1) * 16) = e4m3x8_to_bf16(t.v[i][2], t.v[i][3], v_scale);
             } else {
-                *reinterpret_cast<u32x4*>(kr + (c ^ ks) * 16) = t.k[i];
-                *reinterpret_cast<u32x4*>(vr + (c ^ vs) * 16) = t.v[i];
+                *reinterpret_cast<u32x4*>(kr + k_chunk<D>(r, c) * 16) = t.k[i];
+                *reinterpret_cast<u32x4*>(vr + v_chunk<D>(r, c) * 16) = t.v[i];
             }
         }
         lds_in_order();
@@ -158,7 +156,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(Attention
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) {
                 const int r = 16 * i + q;
-                s[i] = mfma_16x16x32(*reinterpret_cast<const u32x4*>(k_lds + r * kRow + ((4 * j + g) ^ (r & 7)) * 16), qf[j], s[i]);
+                s[i] = mfma_16x16x32(*reinterpret_cast<const u32x4*>(k_lds + r * kRow + k_chunk<D>(r, 4 * j + g) * 16), qf[j], s[i]);
             }
         }
         settle(s[0], s[1]);
@@ -195,7 +193,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(Attention
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = 16 * i + 4 * g + (q >> 2);
-                col[i] = lds_column_of_4(v_lds + r * kRow + ((2 * d + ((q & 3) >> 1)) ^ ((r & 3) << 1)) * 16 + (q & 1) * 8);
+                col[i] = lds_column_of_4(v_lds + r * kRow + v_chunk<D>(r, 2 * d + ((q & 3) >> 1)) * 16 + (q & 1) * 8);
             }
             acc[d] = mfma_16x16x32(u32x4{col[0][0], col[0][1], col[1][0], col[1][1]}, p, acc[d]);
         }

@@ -74,21 +74,34 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
     float m = -INFINITY, l = 0.f;
     const float scale = a.scale * kLog2e;
 
+    // a thread's pieces of a tile: offsets in bytes from the tile's first row, those of rows past the last key the last one's
     u32x4 kr[kLoads], vr[kLoads];
-    const uint16_t* k_base = a.k + (size_t)ks.begin * a.k_stride + (size_t)kv_head * D;
-    const uint16_t* v_base = a.v + (size_t)ks.begin * a.v_stride + (size_t)kv_head * D;
-    auto load = [&](int key0) {
+    uint32_t k_off[kLoads], v_off[kLoads];
+    auto offsets = [&](int rows) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int at = threadIdx.x + 64 * kWaves * i, r = min(key0 + at / kChunks, ks.rows - 1), c = at % kChunks;
-            kr[i] = *reinterpret_cast<const u32x4*>(k_base + (size_t)r * a.k_stride + 8 * c);
-            vr[i] = *reinterpret_cast<const u32x4*>(v_base + (size_t)r * a.v_stride + 8 * c);
+            const int at = threadIdx.x + 64 * kWaves * i;
+            const uint32_t r = min(at / kChunks, rows - 1), c = at % kChunks;
+            k_off[i] = 2 * (r * (uint32_t)a.k_stride + 8 * c);
+            v_off[i] = 2 * (r * (uint32_t)a.v_stride + 8 * c);
+        }
+    };
+    offsets(kKeys);
+    const uint8_t* k_base = reinterpret_cast<const uint8_t*>(a.k + (size_t)ks.begin * a.k_stride + (size_t)kv_head * D);
+    const uint8_t* v_base = reinterpret_cast<const uint8_t*>(a.v + (size_t)ks.begin * a.v_stride + (size_t)kv_head * D);
+    auto load = [&](int key0) {
+        if (key0 + kKeys > ks.rows) offsets(ks.rows - key0);  // the last tile
+        const uint8_t* k = k_base + (size_t)key0 * a.k_stride * 2;
+        const uint8_t* v = v_base + (size_t)key0 * a.v_stride * 2;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            kr[i] = *reinterpret_cast<const u32x4*>(k + k_off[i]);
+            vr[i] = *reinterpret_cast<const u32x4*>(v + v_off[i]);
         }
     };
     // Whether some row of the block does not see all of these keys.  Their values go to LDS without infinities and NaNs, which a weight of 0 does not undo;
     // the rows that do see those get them afterwards.
     auto cut = [&](int key0) { return key0 + kKeys - 1 > row0 + ahead || (a.window && key0 < end - a.window); };
-    // chunk c of row r at c ^ (r % 8) for K, which is read by rows, at c ^ 2 (r % 4) for V, read by columns of four rows
     auto store = [&](int buffer, int key0) {
         if (cut(key0)) {
             auto not_finite = [](uint32_t x) { return ((x & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u); };
@@ -109,13 +122,13 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int at = threadIdx.x + 64 * kWaves * i, r = at / kChunks, c = at % kChunks;
-            *reinterpret_cast<u32x4*>(&lds[buffer][0][r * kRow + (c ^ (r & 7)) * 16]) = kr[i];
-            *reinterpret_cast<u32x4*>(&lds[buffer][1][r * kRow + (c ^ ((r & 3) << 1)) * 16]) = vr[i];
+            *reinterpret_cast<u32x4*>(&lds[buffer][0][r * kRow + k_chunk<D>(r, c) * 16]) = kr[i];
+            *reinterpret_cast<u32x4*>(&lds[buffer][1][r * kRow + v_chunk<D>(r, c) * 16]) = vr[i];
         }
     };
     auto v_column = [&](const uint8_t* v, int key, int d) {  // keys key .. key + 3 (+ 4 in the upper half), the lane's dimension of 32 d ..
         const int i = lane & 15, r = key + 4 * hi + (i >> 2), c = 4 * d + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
-        return lds_column_of_4(v + r * kRow + (c ^ ((r & 3) << 1)) * 16 + (i & 1) * 8);
+        return lds_column_of_4(v + r * kRow + v_chunk<D>(r, c) * 16 + (i & 1) * 8);
     };
     auto compute = [&](int buffer, int key0) {
         const uint8_t* k = lds[buffer][0];
@@ -128,7 +141,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) {
                 const int r = 32 * t + col;
-                s[t] = mfma_32x32x16(*reinterpret_cast<const u32x4*>(k + r * kRow + ((2 * j + hi) ^ (r & 7)) * 16), qf[j], s[t]);
+                s[t] = mfma_32x32x16(*reinterpret_cast<const u32x4*>(k + r * kRow + k_chunk<D>(r, 2 * j + hi) * 16), qf[j], s[t]);
             }
         }
         settle(s[0], s[1]);
@@ -187,7 +200,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
                 const u32x4 weights = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
 #pragma unroll
                 for (int d = 0; d < kDims; ++d) {
-                    const uint32_t x = v_base[(size_t)(key0 + i) * a.v_stride + 32 * d + col], left = mine && (x & 0x7F80u) == 0x7F80u ? x << (e & 1) * 16 : 0u;
+                    const uint32_t x = reinterpret_cast<const uint16_t*>(v_base)[(size_t)(key0 + i) * a.v_stride + 32 * d + col], left = mine && (x & 0x7F80u) == 0x7F80u ? x << (e & 1) * 16 : 0u;
                     u32x4 one;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) one[w] = e >> 1 == w ? left : 0u;
@@ -209,16 +222,17 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
         __syncthreads();
         store(0, begin);
         __syncthreads();
-        int buffer = 0;
-        for (int key0 = begin; key0 < end; key0 += kKeys) {
+        auto step = [&](int buffer, int key0) {  // true: that was the last tile
             const bool more = key0 + kKeys < end;
             if (more) load(key0 + kKeys);
             // whether any row of the wave sees any of these keys
             if (key0 <= wave_row + 31 + ahead && (!a.window || key0 + kKeys > wave_row + ahead - a.window + 1) && wave_row < qs.rows) compute(buffer, key0);
             if (more) store(buffer ^ 1, key0 + kKeys);
             __syncthreads();
-            buffer ^= 1;
-        }
+            return !more;
+        };
+        for (int key0 = begin;; key0 += 2 * kKeys)
+            if (step(0, key0) || step(1, key0 + kKeys)) break;
     }
 
 #pragma unroll
