@@ -74,57 +74,52 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
     float m = -INFINITY, l = 0.f;
     const float scale = a.scale * kLog2e;
 
-    // a thread's pieces of a tile: offsets in bytes from the tile's first row, those of rows past the last key the last one's
-    u32x4 kr[kLoads], vr[kLoads];
+    // a lane's share of a tile: kLoads pieces of 1 KiB to a wave, each linear in LDS; offsets in bytes from the tile's first row, of rows past the last key
+    // the last one's
     uint32_t k_off[kLoads], v_off[kLoads];
     auto offsets = [&](int rows) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int at = threadIdx.x + 64 * kWaves * i;
-            const uint32_t r = min(at / kChunks, rows - 1), c = at % kChunks;
-            k_off[i] = 2 * (r * (uint32_t)a.k_stride + 8 * c);
-            v_off[i] = 2 * (r * (uint32_t)a.v_stride + 8 * c);
+            const int r = (wave * kLoads + i) * (64 / kChunks) + lane / kChunks, c = lane % kChunks;
+            const uint32_t from = min(r, rows - 1);
+            k_off[i] = 2 * (from * (uint32_t)a.k_stride + 8 * k_chunk<D>(r, c));
+            v_off[i] = 2 * (from * (uint32_t)a.v_stride + 8 * v_chunk<D>(r, c));
         }
     };
     offsets(kKeys);
     const uint8_t* k_base = reinterpret_cast<const uint8_t*>(a.k + (size_t)ks.begin * a.k_stride + (size_t)kv_head * D);
     const uint8_t* v_base = reinterpret_cast<const uint8_t*>(a.v + (size_t)ks.begin * a.v_stride + (size_t)kv_head * D);
-    auto load = [&](int key0) {
+    const uint32_t lds_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds[0][0][0]) + wave * kLoads * 1024;
+    auto load = [&](int buffer, int key0) {
         if (key0 + kKeys > ks.rows) offsets(ks.rows - key0);  // the last tile
         const uint8_t* k = k_base + (size_t)key0 * a.k_stride * 2;
         const uint8_t* v = v_base + (size_t)key0 * a.v_stride * 2;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            kr[i] = *reinterpret_cast<const u32x4*>(k + k_off[i]);
-            vr[i] = *reinterpret_cast<const u32x4*>(v + v_off[i]);
+            tile_dma16(k, k_off[i], lds_at + buffer * 2 * kKeys * kRow + i * 1024);
+            tile_dma16(v, v_off[i], lds_at + (buffer * 2 + 1) * kKeys * kRow + i * 1024);
         }
     };
-    // Whether some row of the block does not see all of these keys.  Their values go to LDS without infinities and NaNs, which a weight of 0 does not undo;
-    // the rows that do see those get them afterwards.
+    // Whether some row of the block does not see all of these keys.  Infinities and NaNs among their values, which a weight of 0 does not undo, are then
+    // taken out of LDS; the rows that do see them get them afterwards.
     auto cut = [&](int key0) { return key0 + kKeys - 1 > row0 + ahead || (a.window && key0 < end - a.window); };
-    auto store = [&](int buffer, int key0) {
-        if (cut(key0)) {
-            auto not_finite = [](uint32_t x) { return ((x & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u); };
-            uint32_t any = 0;
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const bool outside = key0 + (int)(threadIdx.x + 64 * kWaves * i) / kChunks >= ks.rows;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    if (outside) vr[i][w] = 0;
-                    const uint32_t off = not_finite(vr[i][w]);
-                    vr[i][w] &= ~off;
-                    any |= off;
-                }
-            }
-            if (any) odd[buffer] = key0;
-        }
+    auto clean = [&](int buffer, int key0) {
+        auto not_finite = [](uint32_t x) { return ((x & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u); };
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int at = threadIdx.x + 64 * kWaves * i, r = at / kChunks, c = at % kChunks;
-            *reinterpret_cast<u32x4*>(&lds[buffer][0][r * kRow + k_chunk<D>(r, c) * 16]) = kr[i];
-            *reinterpret_cast<u32x4*>(&lds[buffer][1][r * kRow + v_chunk<D>(r, c) * 16]) = vr[i];
+            u32x4* at = reinterpret_cast<u32x4*>(&lds[buffer][1][0]) + threadIdx.x + 64 * kWaves * i;
+            u32x4 x = *at;
+            uint32_t off[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) off[w] = not_finite(x[w]);
+            if (off[0] | off[1] | off[2] | off[3]) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) x[w] &= ~off[w];
+                *at = x;
+                odd[buffer] = key0;
+            }
         }
+        __syncthreads();
     };
     auto v_column = [&](const uint8_t* v, int key, int d) {  // keys key .. key + 3 (+ 4 in the upper half), the lane's dimension of 32 d ..
         const int i = lane & 15, r = key + 4 * hi + (i >> 2), c = 4 * d + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
@@ -218,21 +213,16 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
 
     if (begin < end) {
         if (threadIdx.x < 2) odd[threadIdx.x] = -1;
-        load(begin);
-        __syncthreads();
-        store(0, begin);
-        __syncthreads();
-        auto step = [&](int buffer, int key0) {  // true: that was the last tile
-            const bool more = key0 + kKeys < end;
-            if (more) load(key0 + kKeys);
+        load(0, begin);
+        int buffer = 0;
+        for (int key0 = begin; key0 < end; key0 += kKeys) {
+            wait_and_meet<0>();  // the tile is there, and all waves have left the one before it
+            if (key0 + kKeys < end) load(buffer ^ 1, key0 + kKeys);
+            if (cut(key0)) clean(buffer, key0);
             // whether any row of the wave sees any of these keys
             if (key0 <= wave_row + 31 + ahead && (!a.window || key0 + kKeys > wave_row + ahead - a.window + 1) && wave_row < qs.rows) compute(buffer, key0);
-            if (more) store(buffer ^ 1, key0 + kKeys);
-            __syncthreads();
-            return !more;
-        };
-        for (int key0 = begin;; key0 += 2 * kKeys)
-            if (step(0, key0) || step(1, key0 + kKeys)) break;
+            buffer ^= 1;
+        }
     }
 
 #pragma unroll
