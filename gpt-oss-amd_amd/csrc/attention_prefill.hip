@@ -1,5 +1,6 @@
 // Causal attention over packed prompts: out = softmax(scale q K^T, sinks) V, query heads in groups that share a key/value head.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.h"
 #include "kernels.h"
@@ -100,8 +101,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
             tile_dma16(v, v_off[i], lds_at + (buffer * 2 + 1) * kKeys * kRow + i * 1024);
         }
     };
-    // Whether some row of the block does not see all of these keys.  Infinities and NaNs among their values, which a weight of 0 does not undo, are then
-    // taken out of LDS; the rows that do see them get them afterwards.
+    // Whether some row of the block does not see all of these keys.  Infinities and NaNs among their values, which a weight of 0 does not undo, are taken
+    // out of LDS in the careful pass; the rows that do see them get them afterwards.
     auto cut = [&](int key0) { return key0 + kKeys - 1 > row0 + ahead || (a.window && key0 < end - a.window); };
     auto clean = [&](int buffer, int key0) {
         auto not_finite = [](uint32_t x) { return ((x & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u); };
@@ -125,20 +126,19 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
         const int i = lane & 15, r = key + 4 * hi + (i >> 2), c = 4 * d + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
         return lds_column_of_4(v + r * kRow + v_chunk<D>(r, c) * 16 + (i & 1) * 8);
     };
-    auto compute = [&](int buffer, int key0) {
+    auto compute = [&](int buffer, int key0, auto careful) {
         const uint8_t* k = lds[buffer][0];
         const uint8_t* v = lds[buffer][1];
         f32x16 s[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int i = 0; i < 16; ++i) s[0][i] = s[1][i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+        for (int j = 0; j < kSteps; ++j)
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
+            for (int t = 0; t < 2; ++t) {
                 const int r = 32 * t + col;
                 s[t] = mfma_32x32x16(*reinterpret_cast<const u32x4*>(k + r * kRow + k_chunk<D>(r, 2 * j + hi) * 16), qf[j], s[t]);
             }
-        }
         settle(s[0], s[1]);
         if (key0 + kKeys - 1 > wave_row + ahead || (a.window && key0 < wave_row + 31 + ahead - a.window + 1)) {
 #pragma unroll
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
                 const u32x2 x = v_column(v, 16 * j, d), y = v_column(v, 16 * j + 8, d);
                 acc[d] = mfma_32x32x16(u32x4{x[0], x[1], y[0], y[1]}, p[j], acc[d]);
             }
-        if (cut(key0) && odd[buffer] == key0) {  // what was left out, a key at a time, added where it is seen
+        if (decltype(careful)::value && cut(key0) && odd[buffer] == key0) {  // what was left out, a key at a time, added where it is seen
 #pragma unroll
             for (int d = 0; d < kDims; ++d) settle(acc[d]);
             for (int i = 0; i < kKeys && key0 + i < ks.rows; ++i) {
@@ -211,22 +211,41 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
         }
     };
 
-    if (begin < end) {
-        if (threadIdx.x < 2) odd[threadIdx.x] = -1;
+    auto pass = [&](auto careful) {
         load(0, begin);
         int buffer = 0;
         for (int key0 = begin; key0 < end; key0 += kKeys) {
             wait_and_meet<0>();  // the tile is there, and all waves have left the one before it
             if (key0 + kKeys < end) load(buffer ^ 1, key0 + kKeys);
-            if (cut(key0)) clean(buffer, key0);
+            if (decltype(careful)::value && cut(key0)) clean(buffer, key0);
             // whether any row of the wave sees any of these keys
-            if (key0 <= wave_row + 31 + ahead && (!a.window || key0 + kKeys > wave_row + ahead - a.window + 1) && wave_row < qs.rows) compute(buffer, key0);
+            if (key0 <= wave_row + 31 + ahead && (!a.window || key0 + kKeys > wave_row + ahead - a.window + 1) && wave_row < qs.rows)
+                compute(buffer, key0, careful);
             buffer ^= 1;
         }
-    }
-
 #pragma unroll
-    for (int d = 0; d < kDims; ++d) settle(acc[d]);
+        for (int d = 0; d < kDims; ++d) settle(acc[d]);
+    };
+    if (begin < end) {
+        pass(std::false_type{});
+        // A value that is not finite under a weight of 0 has made a NaN of its row's sum.  So has one that the row sees: the careful pass tells them apart.
+        float sum = 0.f;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum = fmaf(acc[d][i], 0.f, sum);  // 0 if all are finite
+        if (__syncthreads_or(!(sum == 0.f))) {
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+            m = -INFINITY;
+            l = 0.f;
+            if (threadIdx.x < 2) odd[threadIdx.x] = -1;
+            offsets(kKeys);
+            pass(std::true_type{});
+        }
+    }
     if (a.sinks) {
         const float sink = bf16_bits_to_f32(a.sinks[head]) * kLog2e, most = fmaxf(m, sink), base = most == -INFINITY ? 0.f : most;
         const float down = __builtin_amdgcn_exp2f(m - base);
