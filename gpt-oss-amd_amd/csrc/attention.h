@@ -92,4 +92,21 @@ MOE_DEVICE bool find_item(int n, int j, F count, int& seq, int& within) {
     return false;
 }
 
+// The same from the last item backwards: item j of the reversed order.
+template <class F>
+MOE_DEVICE bool find_last_item(int n, int j, F count, int& seq, int& within) {
+    const int lane = threadIdx.x & 63;
+    if (n <= 64) {  // one look at the counts
+        const int c = lane < n ? count(lane) : 0, upto = wave_prefix_sum(c), at = __builtin_amdgcn_readlane(upto, 63) - 1 - j;
+        const uint64_t past = __ballot(upto > at);
+        if (at < 0) return false;
+        seq = __builtin_ctzll(past);
+        within = at - (__builtin_amdgcn_readlane(upto, seq) - __builtin_amdgcn_readlane(c, seq));
+        return true;
+    }
+    int all = 0;
+    for (int base = 0; base < n; base += 64) all += wave_sum(base + lane < n ? count(base + lane) : 0);
+    return j < all && find_item(n, all - 1 - j, count, seq, within);
+}
+
 }  // namespace moe
