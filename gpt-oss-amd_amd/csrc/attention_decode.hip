@@ -38,31 +38,92 @@ MOE_DEVICE float mx_scale(uint32_t b) { return __uint_as_float(b == 255u ? 0x7FC
 }  // namespace
 
 // Item (sequence, piece of its keys, KV head, 16 of the query heads that share it) to a block; pieces are as long as makes about a.pieces of
-// them per head over all sequences, so that the longest sequence does not hold up the others.  A wave takes every fourth tile of 32 keys:
+// them per head over all sequences, so that the longest sequence does not hold up the others; the whole pieces come first, the shorter ones end the launch.  A wave takes every fourth tile of 32 keys:
 // whole rows of K and V into registers a tile ahead, through its own LDS into the matrix operands.  S^T = K Q^T puts a query head into
 // a lane column, so that its running maximum and sum are a lane's and P^T is the second product's operand as it stands: O^T = V^T P^T, with
 // V^T read as columns from LDS.  P is rounded to bf16 for that product (half a step is up to 2^-8 of a weight, as that of the bf16 result); its sum is
 // taken before that, in fp32.  Statistics are in powers of two: s' = scale log2(e) q.k.
 template <int D, bool MX>
-__global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(AttentionDecodeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 2) void attention_decode_kernel(AttentionDecodeArgs a) {
     constexpr int kRow = 2 * D, kSteps = D / 32, kDims = D / 16;
     using Loads = TileLoads<D, MX>;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane & 15, g = lane >> 4;
     const int G = a.n_heads / a.n_kv_heads, group_tiles = ceil_div(G, 16);
     const int h = blockIdx.x % a.n_kv_heads, rest = blockIdx.x / a.n_kv_heads, gt = rest % group_tiles, item = rest / group_tiles;
 
-    // the piece
+    // the piece; up to 512 sequences are looked at once, eight to a lane
+    constexpr int kHeld = 8;
+    const bool held = a.batch <= 64 * kHeld;
+    auto keys_of = [&](int s) { return seen_of(a, s).keys(); };
+    int mine[kHeld];
     double total = 0.0;  // keys of all sequences, exact
-    for (int base = 0; base < a.batch; base += 64) total += wave_sum(base + lane < a.batch ? (double)seen_of(a, base + lane).keys() : 0.0);
+    if (held) {
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            mine[i] = 0;
+            if (64 * i >= a.batch) continue;
+            if (64 * i + lane < a.batch) mine[i] = keys_of(64 * i + lane);
+            sum += (double)mine[i];
+        }
+        total = wave_sum(sum);
+    } else {
+        for (int base = 0; base < a.batch; base += 64) total += wave_sum(base + lane < a.batch ? (double)keys_of(base + lane) : 0.0);
+    }
     const long long even = (long long)(total / a.pieces) + 1;
     constexpr int kStep = kWaves * kTile;
     const int piece = (int)min(max((even + kStep - 1) / kStep * kStep, (long long)a.min_piece), 1ll << 30);
-    int b, part;
-    auto pieces_of = [&](int s) { return max(1, ceil_div(seen_of(a, s).keys(), piece)); };
-    if (!find_item(a.batch, item, pieces_of, b, part)) return;
+    // items: the whole pieces of all sequences, then what is left of each
+    int b = 0, part, n_whole = 0, first_part = 0, all_whole = 0;
+    if (held) {
+        int n[kHeld], upto[kHeld];
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            if (64 * i >= a.batch) continue;
+            n[i] = mine[i] / piece;
+            upto[i] = all_whole + wave_prefix_sum(n[i]);
+            all_whole = __builtin_amdgcn_readlane(upto[i], 63);
+        }
+        if (item - all_whole >= a.batch) return;
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            if (64 * i >= a.batch || found) continue;
+            const uint64_t past = item < all_whole ? __ballot(upto[i] > item) : 64 * i + 63 >= item - all_whole ? 1ull << ((item - all_whole) & 63) : 0;
+            if (past) {
+                const int at = __builtin_ctzll(past);
+                found = true;
+                b = 64 * i + at;
+                n_whole = __builtin_amdgcn_readlane(n[i], at);
+                first_part = __builtin_amdgcn_readlane(upto[i], at) - n_whole;
+            }
+        }
+    } else {
+        auto whole_of = [&](int s) { return keys_of(s) / piece; };
+        for (int base = 0; base < a.batch; base += 64) all_whole += wave_sum(base + lane < a.batch ? whole_of(base + lane) : 0);
+        if (item - all_whole >= a.batch) return;
+        if (item < all_whole) {
+            find_item(a.batch, item, whole_of, b, part);
+            first_part = item - part;
+        } else {
+            b = item - all_whole;
+            for (int base = 0; base < b; base += 64) first_part += wave_sum(base + lane < b ? whole_of(base + lane) : 0);
+        }
+        n_whole = __builtin_amdgcn_readfirstlane(whole_of(b));
+    }
+    part = item < all_whole ? item - first_part : n_whole;
     const Seen seen = seen_of(a, b);
-    const int n_parts = max(1, ceil_div(seen.keys(), piece));
+    const bool left = n_whole == 0 || n_whole * piece < seen.keys();
+    const int n_parts = n_whole + (left ? 1 : 0);
     const int begin = seen.start + part * piece, end = min(seen.len, begin + piece);
+    if (item >= all_whole) {
+        if (h == 0 && gt == 0 && threadIdx.x == 0) {
+            a.plan[3 * b] = first_part;
+            a.plan[3 * b + 1] = n_whole;
+            a.plan[3 * b + 2] = left ? item : -1;
+        }
+        if (!left) return;
+    }
 
     __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * 2 * kTile * kRow];
     uint8_t* k_lds = lds + wave * 2 * kTile * kRow;
@@ -260,10 +321,6 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(Attention
             if (d == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{most, sum};
         }
     }
-    if (part == 0 && h == 0 && gt == 0 && threadIdx.x == 0) {
-        a.plan[2 * b] = item;
-        a.plan[2 * b + 1] = n_parts;
-    }
 }
 
 // The parts of sequences that were cut, joined: a block to a sequence and some heads; a row of D floats to D / 4 lanes, which take every kAtOnce-th part with
@@ -271,7 +328,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(Attention
 template <int D>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionDecodeArgs a, int heads_per_block) {
     constexpr int kLanes = D / 4, kAtOnce = 256 / kLanes;
-    const int b = blockIdx.x, first = a.plan[2 * b], n = a.plan[2 * b + 1];
+    const int b = blockIdx.x, first = a.plan[3 * b], n_whole = a.plan[3 * b + 1], left = a.plan[3 * b + 2], n = n_whole + (left >= 0 ? 1 : 0);
     if (n == 1) return;
     __shared__ f32x2 stats[kAtOnce];
     __shared__ __attribute__((aligned(16))) float rows[kAtOnce][D];
@@ -281,7 +338,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionDecodeArgs
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int i = slot; i < n; i += kAtOnce) {
-            const size_t at = (size_t)(first + i) * a.n_heads + head;
+            const size_t at = (size_t)(i < n_whole ? first + i : left) * a.n_heads + head;
             const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * at);
             const f32x4 row = *reinterpret_cast<const f32x4*>(a.part_o + at * D + d);
             const float now = fmaxf(most, ml[0]), base = now == -INFINITY ? 0.f : now;
@@ -325,7 +382,7 @@ size_t attention_decode_workspace(int batch, int n_heads, int n_kv_heads, int he
     int pieces;
     const size_t items = most_items(batch, n_kv_heads, group_tiles_of(n_heads, n_kv_heads), &pieces);
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-    *ml = up((size_t)batch * 8);
+    *ml = up((size_t)batch * 12);
     *o = *ml + up(items * n_heads * 8);
     return *o + up(items * n_heads * head_dim * 4);
 }

@@ -232,7 +232,7 @@ struct RopeKvArgs {
 int launch_rope_kv_write(const RopeKvArgs& a, bool bf16_rows, hipStream_t stream);
 
 // ---- attention_decode.hip ----------------------------------------------------------------------
-constexpr int kDecodePieces = 768;  // blocks that a launch aims at: three to a compute unit, which are resident at once
+constexpr int kDecodePieces = 512;  // blocks that a launch aims at, two to a compute unit: with fewer parts there is less to join
 struct AttentionDecodeArgs {
     uint16_t* out;
     const uint16_t* q;
@@ -243,7 +243,7 @@ struct AttentionDecodeArgs {
     const int* page_table;    // [batch, max_pages]
     const int* lengths;
     const uint16_t* sinks;    // or nullptr
-    int* plan;                // workspace: [batch, 2] first part, parts
+    int* plan;                // workspace: [batch, 3] first whole part, whole parts, the shorter one or -1
     float* part_ml;           // [parts, n_heads, 2]
     float* part_o;            // [parts, n_heads, head_dim]
     int batch, n_heads, n_kv_heads, max_pages, n_pages, page_shift, window;

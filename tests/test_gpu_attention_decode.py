@@ -87,7 +87,8 @@ def test_lengths_and_heads(pkg, dev, D, fmt, Hq, Hkv, page, window, sinks):
 
 @pytest.mark.parametrize("lens,Hq,Hkv,D,fmt,page,window", [
     ([20000], 8, 1, 64, "bf16", 64, 0), ([9001], 16, 2, 128, "mx8", 32, 0), ([5000, 1, 700, 0, 64, 3333], 8, 2, 64, "mx8", 16, 0),
-    ([6000, 40], 4, 2, 128, "bf16", 256, 2500), ([1] * 70 + [4000] + [3] * 70, 2, 1, 64, "bf16", 16, 0), ([300] * 200, 2, 2, 64, "bf16", 16, 0)])
+    ([6000, 40], 4, 2, 128, "bf16", 256, 2500), ([1] * 70 + [4000] + [3] * 70, 2, 1, 64, "bf16", 16, 0), ([300] * 200, 2, 2, 64, "bf16", 16, 0),
+    ([5] * 300 + [3000] + [40] * 100, 2, 1, 64, "mx8", 16, 0), ([5] * 520 + [4100, 0] + [40] * 100, 2, 1, 64, "bf16", 16, 0)])
 def test_long_ones_in_parts(pkg, dev, lens, Hq, Hkv, D, fmt, page, window):
     print(lens[:3], Hq, Hkv, D, fmt, page, window, flush=True)
     for sinks in (False, True):
