@@ -138,16 +138,20 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
                 s[t] = mfma_32x32x16(*reinterpret_cast<const u32x4*>(k + r * kRow + k_chunk<D>(r, 2 * j + hi) * 16), qf[j], s[t]);
             }
         settle(s[0], s[1]);
-        auto hide = [&](auto hidden) {
+        if (key0 + kKeys - 1 > wave_row + ahead || (a.window && key0 < wave_row + 31 + ahead - a.window + 1)) {
+            // a bit a key that the row sees, spread over its score; comparisons would each wait for the one before it to leave the condition register
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t) {
+                const int from = first - key0 - 32 * t, to = last - key0 - 32 * t;  // of keys 0 .. 31
+                const uint32_t upto = to < 0 ? 0u : to >= 31 ? ~0u : (2u << to) - 1u, since = from <= 0 ? ~0u : from > 31 ? 0u : ~0u << from;
+                const uint32_t seen = (upto & since) >> 4 * hi;
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[t][i] = hidden(32 * t + 8 * (i / 4) + i % 4) ? -INFINITY : s[t][i];
-        };
-        const int at_last = last - key0 - 4 * hi, at_first = first - key0 - 4 * hi;
-        if (key0 + kKeys - 1 > wave_row + ahead) hide([&](int key) { return key > at_last; });
-        if (a.window && key0 < wave_row + 31 + ahead - a.window + 1) hide([&](int key) { return key < at_first; });
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)seen, 8 * (i / 4) + i % 4, 1);
+                    s[t][i] = __uint_as_float((keep & __float_as_uint(s[t][i])) | (~keep & 0xFF800000u));
+                }
+            }
+        }
         u32x4 p[4];
         auto weigh = [&](float base) {
             float sum[2] = {0.f, 0.f};
