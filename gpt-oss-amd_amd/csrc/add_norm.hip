@@ -40,17 +40,9 @@ MOE_DEVICE void f32_scale(uint32_t bits, double amax, float& scale, double& mult
     mult = 448.0 * fma(fma(-a, r, 1.0), r, r);
 }
 
-// y * mult with the bits that fp32 has no room for gathered in its last one (odd if anything was cut off), so that the rounding to e4m3 is the
-// only one: a value next to the middle of two codes does not become it.
-MOE_DEVICE float product_to_odd(double y, double mult) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, y * mult);
-    const uint32_t lo = (uint32_t)b;
-    const uint32_t odd = min(lo & 0x1FFFFFFFu, 1u) << 29;
-    return (float)__builtin_bit_cast(double, (b & 0xFFFFFFFFE0000000ull) | odd);
-}
 MOE_DEVICE uint32_t to_e4m3x4(const Double4& y, double mult) {
-    int v = __builtin_amdgcn_cvt_pk_fp8_f32(product_to_odd(y.x, mult), product_to_odd(y.y, mult), 0, false);
-    v = __builtin_amdgcn_cvt_pk_fp8_f32(product_to_odd(y.z, mult), product_to_odd(y.w, mult), v, true);
+    int v = __builtin_amdgcn_cvt_pk_fp8_f32(to_odd(y.x * mult), to_odd(y.y * mult), 0, false);
+    v = __builtin_amdgcn_cvt_pk_fp8_f32(to_odd(y.z * mult), to_odd(y.w * mult), v, true);
     return (uint32_t)v;
 }
 

@@ -38,11 +38,13 @@ MOE_DEVICE float mx_scale(uint32_t b) { return __uint_as_float(b == 255u ? 0x7FC
 }  // namespace
 
 // Item (sequence, piece of its keys, KV head, 16 of the query heads that share it) to a block; pieces are as long as makes about a.pieces of
-// them per head over all sequences, so that the longest sequence does not hold up the others; the whole pieces come first, the shorter ones end the launch.  A wave takes every fourth tile of 32 keys:
-// whole rows of K and V into registers a tile ahead, through its own LDS into the matrix operands.  S^T = K Q^T puts a query head into
-// a lane column, so that its running maximum and sum are a lane's and P^T is the second product's operand as it stands: O^T = V^T P^T, with
-// V^T read as columns from LDS.  P is rounded to bf16 for that product (half a step is up to 2^-8 of a weight, as that of the bf16 result); its sum is
-// taken before that, in fp32.  Statistics are in powers of two: s' = scale log2(e) q.k.
+// them per head over all sequences, so that the longest sequence does not hold up the others; the whole pieces come first, the shorter ones end the launch.
+// A wave takes every fourth tile of 32 keys: whole rows of K and V into registers two tiles ahead, past the caches (128 sequences of 4096 keys in 8 bits
+// 201 : 178 us), through its own LDS into the matrix operands: loads in the operands' order would touch a line in two or four instructions.  S^T = K Q^T puts
+// a query head into a lane column, so that its running maximum and sum are a lane's and P^T is the second product's operand as it stands: O^T = V^T P^T,
+// with V^T read as columns from LDS.  P goes into that product as two bf16 parts, to 2^-16 of a weight: the matrix units have time.  Statistics are
+// in powers of two: s' = scale log2(e) q.k.
+// Bound by HBM: 128 sequences of 4096 keys, 8 heads of 128 in 8 bits 178 us, 6.2 TB/s; one of 131072, 8 heads of 64, 44 us, 6.0 TB/s, and 4.7 for the join.
 template <int D, bool MX>
 __global__ __launch_bounds__(64 * kWaves, 2) void attention_decode_kernel(AttentionDecodeArgs a) {
     constexpr int kRow = 2 * D, kSteps = D / 32, kDims = D / 16;
@@ -237,7 +239,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_decode_kernel(Attent
         l *= down;
 #pragma unroll
         for (int d = 0; d < kDims; ++d) acc[d] *= down;
-        u32x4 p;
+        u32x4 p, rest;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -245,8 +247,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_decode_kernel(Attent
                 s[i][j] = __builtin_amdgcn_exp2f(s[i][j] - base);
                 l += s[i][j];
             }
-            p[2 * i] = pack_bf16x2(s[i][0], s[i][1]);
-            p[2 * i + 1] = pack_bf16x2(s[i][2], s[i][3]);
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                const uint32_t w = pack_bf16x2(s[i][j], s[i][j + 1]);
+                p[2 * i + j / 2] = w;
+                rest[2 * i + j / 2] = pack_bf16x2(s[i][j] - __uint_as_float(w << 16), s[i][j + 1] - __uint_as_float(w & 0xFFFF0000u));
+            }
         }
 #pragma unroll
         for (int d = 0; d < kDims; ++d) {
@@ -256,7 +262,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_decode_kernel(Attent
                 const int r = 16 * i + 4 * g + (q >> 2);
                 col[i] = lds_column_of_4(v_lds + r * kRow + v_chunk<D>(r, 2 * d + ((q & 3) >> 1)) * 16 + (q & 1) * 8);
             }
-            acc[d] = mfma_16x16x32(u32x4{col[0][0], col[0][1], col[1][0], col[1][1]}, p, acc[d]);
+            const u32x4 values = {col[0][0], col[0][1], col[1][0], col[1][1]};
+            acc[d] = mfma_16x16x32(values, p, acc[d]);
+            acc[d] = mfma_16x16x32(values, rest, acc[d]);
         }
         lds_in_order();
     };

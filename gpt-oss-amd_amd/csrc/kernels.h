@@ -232,7 +232,9 @@ struct RopeKvArgs {
 int launch_rope_kv_write(const RopeKvArgs& a, bool bf16_rows, hipStream_t stream);
 
 // ---- attention_decode.hip ----------------------------------------------------------------------
-constexpr int kDecodePieces = 512;  // blocks that a launch aims at, two to a compute unit: with fewer parts there is less to join
+// Blocks that a launch aims at, two to a compute unit.  us with 512 : 768 : 1024: one sequence of 131072 keys 49.3 : 51.2 : 53.5, 64 ragged ones up to
+// 16384 48.3 : 49.9 : 48.7, 200 up to 3000, heads of 128, 47.7 : 49.7 : 49.5.
+constexpr int kDecodePieces = 512;
 struct AttentionDecodeArgs {
     uint16_t* out;
     const uint16_t* q;

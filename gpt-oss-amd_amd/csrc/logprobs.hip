@@ -277,8 +277,10 @@ MOE_DEVICE void write_row(const LogprobArgs& a, int row, float token, const Sums
 
 // A block to a row or one of `parts` of it (several where there are few rows); a wave takes every kWaves-th step of 512 values.  One pass: the running
 // maximum is the wave's, so that most steps change neither it nor the list of the largest values, which is what one comparison of each lane's
-// largest value asks, and cost a product, an exponential and two additions a value.  Values before the first 16-byte border and behind the
-// last whole step are read one by one, by the last wave while its first steps come.  Bound by HBM.
+// largest value asks, and cost a difference, an exponential and two sums a value.  Values before the first 16-byte border and behind the
+// last whole step are read one by one, by the last wave while its first steps come.  Past the last-level cache rows are read past it.
+// Bound by HBM and by its arithmetic: 1000 bf16 rows of 200000 with 5 alternatives 78 to 83 us, 5 TB/s (without the entropy 75, without any sums 70); fp32
+// rows of 131072 with 20 89 us, 5.9 TB/s.  One row of 131072 with 20 alternatives 10.8 us, 5.9 and 4.9 of them the two launches.
 template <class T, bool NT>
 __global__ __launch_bounds__(64 * kWaves) void logprob_kernel(LogprobArgs a, int parts, int part_len) {
     constexpr int kVec = 16 / sizeof(T);  // values of a load
@@ -375,7 +377,8 @@ __global__ __launch_bounds__(64 * kWaves) void logprob_join_kernel(LogprobArgs a
     if (threadIdx.x < 64) write_row(a, row, token, s, list.mine);
 }
 
-// Parts of a row: about kBlocks blocks where there are fewer rows.
+// Parts of a row: about kBlocks blocks where there are fewer rows.  A wave's first list costs it as much as ten steps.  us with 512 : 1024 : 2048 blocks:
+// 1000 rows of 131072 90 : 99 : 111, 100 rows 33 : 34 : 37.
 constexpr int kBlocks = 512;
 static int parts_of(int n_tokens, int vocab) {
     return std::min(ceil_div(kBlocks, n_tokens), ceil_div(vocab, kFewest));

@@ -32,6 +32,15 @@ MOE_DEVICE uint32_t mx_scale_byte(uint32_t amax) {
     return (uint32_t)max(b, 1);
 }
 
+// v in fp32 with the bits that there is no room for gathered in the last one (odd if anything was cut off), so that the rounding to fewer bits that follows is
+// the only one: a value next to the middle of two codes does not become it.
+MOE_DEVICE float to_odd(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)b;
+    const uint32_t odd = min(lo & 0x1FFFFFFFu, 1u) << 29;
+    return (float)__builtin_bit_cast(double, (b & 0xFFFFFFFFE0000000ull) | odd);
+}
+
 // e4m3 values times a power of two (its exponent counts: the bits of 0 are 2^-127), to bf16: exact, with three mantissa bits, but for denormals.
 MOE_DEVICE u32x4 e4m3x8_to_bf16(uint32_t lo, uint32_t hi, float scale) {
     u32x4 v;

@@ -349,12 +349,12 @@ typedef struct moe_kv_cache {
 /* Rotary embedding and cache write.  qkv holds n_tokens rows, `stride` elements apart, of n_heads queries, n_kv_heads keys and n_kv_heads values of
  * head_dim each, fp32 or bf16 (qkv_type MOE_ROWS_*).  Of every query and key the first rotary_dim values turn: with p = positions[token],
  * i < rotary_dim / 2, a = p * inv_freq[i] (exact, in fp64), u = x[i], v = x[i + rotary_dim / 2]:
- *   x[i] = scale (u cos a - v sin a),  x[i + rotary_dim / 2] = scale (v cos a + u sin a)   in fp32, cos and sin to 2^-22
+ *   x[i] = scale (u cos a - v sin a),  x[i + rotary_dim / 2] = scale (v cos a + u sin a)   in fp32, cos and sin to 2^-22; in fp64 for an 8-bit cache
  * Then what is asked for, at least one:
  *   q, k, v   [n_tokens, n_heads or n_kv_heads, head_dim] bf16, each or NULL (k and v for moe_attention_prefill)
  *   cache     keys and values of token t to slot slots[t], or nowhere if that is not in [0, n_pages * page_size); no other slot changes.  The slots of a
  *             call have to differ.  In 8 bits: per 32 values the smallest power of two, from 2^-126, that leaves the largest at 448 or below,
- *             codes rounded to nearest even from fp32; a group with an infinity or a NaN has a NaN for its scale and for every code
+ *             codes the nearest (ties to even); a group with an infinity or a NaN has a NaN for its scale and for every code
  * cache and slots both or neither.  rotary_dim <= head_dim, a multiple of 8 (of 64 with an 8-bit cache), 0 for none (inv_freq may be NULL);
  * n_heads <= 1024; stride >= (n_heads + 2 n_kv_heads) head_dim and a multiple of 4; n_tokens < 2^31 - 255; qkv, q, k, v 16-byte aligned, the
  * rest 4-byte.  No output may overlap an input. */
@@ -366,7 +366,8 @@ MOE_API int moe_rope_kv_write(const void* qkv, int qkv_type, long long stride, c
  * j % page_size of page page_table[b, j / page_size]; its query, the last of them, sees the keys j >= lengths[b] - window (all with window 0).
  * Query heads g, g + 1, .. share a key/value head: head h reads key/value head h / (n_heads / n_kv_heads).
  *   s[j] = scale q . k[j],  out = sum_j exp(s[j]) v[j] / (sum_j exp(s[j]) + exp(sinks[h]))    (without sinks: without their term)
- * A query that sees nothing has zeros.  Products of bf16 values, sums and statistics in fp32, weights rounded to bf16; the result is rounded once.
+ * A query that sees nothing has zeros.  Products of bf16 values, sums and statistics in fp32, weights exp(s) to 2^-16; the result is rounded once.
+ * What is not finite among the keys and values that a query sees makes NaNs or infinities of its results.
  * A page number outside [0, n_pages) is a page without keys, and page numbers behind a sequence's last key are not looked at: a table may hold
  * anything there, as may the slots.  Deterministic, but the sum over keys is cut into pieces that depend on all the lengths of a call.
  * q, out [batch, n_heads, head_dim] bf16, page_table [batch, max_pages], lengths [batch], sinks [n_heads] bf16 or NULL.  n_heads <= 1024, a multiple of
@@ -380,7 +381,7 @@ MOE_API int moe_attention_decode(moe_bf16_t* out, const moe_bf16_t* q, const moe
 
 /* Causal attention over prompts packed one after another: sequence s has the query rows q_starts[s] .. q_starts[s + 1] - 1 of total_q and the key and value
  * rows k_starts[s] .. k_starts[s + 1] - 1 of total_k.  Its queries are its last positions: query i of n sees key j of m if j <= i + m - n and, with
- * a window, j > i + m - n - window.  The rest as moe_attention_decode.  Rows that belong to no sequence are not written.  What one row
+ * a window, j > i + m - n - window.  The rest as moe_attention_decode, with weights rounded to bf16.  Rows that belong to no sequence are not written.  What one row
  * sees does not depend on keys that it does not see, whatever these and their values hold; a row's result does not depend on other sequences.
  * q, out [total_q, n_heads, head_dim], k, v [total_k, n_kv_heads, head_dim] bf16, *_stride elements from token to token (at least a token's, a
  * multiple of 8; k_stride, v_stride <= 2^24); starts ascending (what lies outside the rows is cut off).  head_dim 64 or 128; n_seqs <= 65535; total_q * n_heads < 2^30; all
