@@ -681,7 +681,7 @@ int moe_attention_decode(moe_bf16_t* out, const moe_bf16_t* q, const moe_kv_cach
     char* ws = static_cast<char*>(workspace);
     return launch_attention_decode({out, q, cache->k, cache->v, cache->k_scales, cache->v_scales, page_table, lengths, sinks, reinterpret_cast<int*>(ws),
                                     reinterpret_cast<float*>(ws + ml), reinterpret_cast<float*>(ws + o), batch, n_heads, cache->n_kv_heads, max_pages,
-                                    cache->n_pages, log2_of(cache->page_size), window, scale, 0, 0},
+                                    cache->n_pages, log2_of(cache->page_size), window, scale, 0, 0, 0},
                                    cache->head_dim, as_stream(stream));
 }
 
@@ -695,11 +695,11 @@ int moe_attention_prefill(moe_bf16_t* out, const moe_bf16_t* q, const moe_bf16_t
     if (std::min(out_stride, q_stride) < (long long)n_heads * head_dim || std::min(k_stride, v_stride) < (long long)n_kv_heads * head_dim) return MOE_ERR_SHAPE;
     if ((out_stride | q_stride | k_stride | v_stride) % 8 != 0) return MOE_ERR_SHAPE;
     if (n_seqs > 65535 || (long long)total_q * n_heads >= (1 << 30)) return MOE_ERR_LIMIT;
-    if (std::max(k_stride, v_stride) > (1 << 24)) return MOE_ERR_LIMIT;  // 64 rows within 32 bits of bytes
+    if (std::max(k_stride, v_stride) > (1 << 23)) return MOE_ERR_LIMIT;  // 64 rows within 31 bits of bytes
     if (bad_scale(scale)) return MOE_ERR_FORMAT;
     if (misaligned({out, q, k, v}, 16) || misaligned({q_starts, k_starts}, 4) || misaligned({sinks}, 2)) return MOE_ERR_ALIGN;
     return launch_attention_prefill({out, q, k, v, q_starts, k_starts, sinks, out_stride, q_stride, k_stride, v_stride, n_seqs, total_q, total_k, n_heads,
-                                     n_kv_heads, window, scale},
+                                     n_kv_heads, window, scale, 0},
                                     head_dim, as_stream(stream));
 }
 

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_decode_kernel(Attent
     using Loads = TileLoads<D, MX>;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane & 15, g = lane >> 4;
     const int G = a.n_heads / a.n_kv_heads, group_tiles = ceil_div(G, 16);
-    const int h = blockIdx.x % a.n_kv_heads, rest = blockIdx.x / a.n_kv_heads, gt = rest % group_tiles, item = rest / group_tiles;
+    const int block = a.first_block + blockIdx.x, h = block % a.n_kv_heads, rest = block / a.n_kv_heads, gt = rest % group_tiles, item = rest / group_tiles;
 
     // the piece; up to 512 sequences are looked at once, eight to a lane
     constexpr int kHeld = 8;
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_decode_kernel(Attent
     }
     const long long even = (long long)(total / a.pieces) + 1;
     constexpr int kStep = kWaves * kTile;
-    const int piece = (int)min(max((even + kStep - 1) / kStep * kStep, (long long)a.min_piece), 1ll << 30);
+    const int piece = (int)min(max((even + kStep - 1) / kStep * kStep, (long long)a.min_piece), (1ll << 30) + kStep);
     // items: the whole pieces of all sequences, then what is left of each
     int b = 0, part, n_whole = 0, first_part = 0, all_whole = 0;
     if (held) {
@@ -398,15 +398,18 @@ size_t attention_decode_workspace(int batch, int n_heads, int n_kv_heads, int he
 int launch_attention_decode(AttentionDecodeArgs a, int head_dim, hipStream_t stream) {
     const int group_tiles = group_tiles_of(a.n_heads, a.n_kv_heads);
     const int items = most_items(a.batch, a.n_kv_heads, group_tiles, &a.pieces);
-    const dim3 grid((unsigned)(items * a.n_kv_heads * group_tiles));
+    const int blocks = items * a.n_kv_heads * group_tiles, at_once = (int)(kMostThreads / (64 * kWaves));
     const long long room = (long long)a.max_pages << a.page_shift;
     const long long most = a.window ? std::min<long long>(room, (long long)a.window + kTile - 1) : room;
     a.min_piece = most <= 256 ? 256 : 128;  // a short window is one piece: no parts to join
     const bool join = most > a.min_piece;
     auto run = [&](auto kernel, auto joiner) {
-        hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, stream, a);
-        int rc = launch_status();
-        if (rc || !join) return rc;
+        for (a.first_block = 0; a.first_block < blocks; a.first_block += at_once) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(at_once, blocks - a.first_block)), dim3(64 * kWaves), 0, stream, a);
+            const int rc = launch_status();
+            if (rc) return rc;
+        }
+        if (!join) return (int)MOE_OK;
         const int per_block = std::max(1, ceil_div(a.batch * std::min(a.n_heads, 256), 2048));
         hipLaunchKernelGGL(joiner, dim3((unsigned)a.batch, (unsigned)ceil_div(a.n_heads, per_block)), dim3(256), 0, stream, a, per_block);
         return launch_status();

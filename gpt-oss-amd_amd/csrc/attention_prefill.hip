@@ -39,14 +39,15 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5;
 
     // heads of a group on one XCD (blocks go to them in turn), where its L2 holds their keys
+    const int block = a.first_block + blockIdx.x;
     int head, rank;
     if (a.n_heads % 8 == 0) {
-        const int each = a.n_heads / 8, at = blockIdx.x / 8;
-        head = blockIdx.x % 8 * each + at % each;
+        const int each = a.n_heads / 8, at = block / 8;
+        head = block % 8 * each + at % each;
         rank = at / each;
     } else {
-        head = blockIdx.x % a.n_heads;
-        rank = blockIdx.x / a.n_heads;
+        head = block % a.n_heads;
+        rank = block / a.n_heads;
     }
     auto tiles_of = [&](int s) { return ceil_div(span_of(a.q_starts, s, a.total_q).rows, kRows); };
     int seq, tile;
@@ -282,12 +283,17 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
     }
 }
 
-int launch_attention_prefill(const AttentionPrefillArgs& a, int head_dim, hipStream_t stream) {
-    const long long blocks = ((long long)a.total_q / kRows + std::min(a.n_seqs, a.total_q)) * a.n_heads;  // as many as there can be
-    if (blocks > 0x7FFFFFFFll / (64 * kWaves)) return MOE_ERR_LIMIT;
-    if (head_dim == 64) hipLaunchKernelGGL(attention_prefill_kernel<64>, dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream, a);
-    else hipLaunchKernelGGL(attention_prefill_kernel<128>, dim3((unsigned)blocks), dim3(64 * kWaves), 0, stream, a);
-    return launch_status();
+int launch_attention_prefill(AttentionPrefillArgs a, int head_dim, hipStream_t stream) {
+    // as many as there can be; below 2^30 rows of heads it is less than 2^27
+    const int blocks = (a.total_q / kRows + std::min(a.n_seqs, a.total_q)) * a.n_heads, at_once = (int)(kMostThreads / (64 * kWaves));
+    for (a.first_block = 0; a.first_block < blocks; a.first_block += at_once) {
+        const dim3 grid((unsigned)std::min(at_once, blocks - a.first_block));
+        if (head_dim == 64) hipLaunchKernelGGL(attention_prefill_kernel<64>, grid, dim3(64 * kWaves), 0, stream, a);
+        else hipLaunchKernelGGL(attention_prefill_kernel<128>, grid, dim3(64 * kWaves), 0, stream, a);
+        const int rc = launch_status();
+        if (rc) return rc;
+    }
+    return MOE_OK;
 }
 
 }  // namespace moe

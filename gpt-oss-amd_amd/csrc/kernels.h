@@ -250,7 +250,8 @@ struct AttentionDecodeArgs {
     float* part_o;            // [parts, n_heads, head_dim]
     int batch, n_heads, n_kv_heads, max_pages, n_pages, page_shift, window;
     float scale;
-    int pieces, min_piece;    // set by the launcher
+    int pieces, min_piece;    // set by the launcher, as
+    int first_block;          // the blocks of launches before this one
 };
 size_t attention_decode_workspace(int batch, int n_heads, int n_kv_heads, int head_dim, size_t* ml, size_t* o);
 int launch_attention_decode(AttentionDecodeArgs a, int head_dim, hipStream_t stream);
@@ -267,8 +268,9 @@ struct AttentionPrefillArgs {
     long long out_stride, q_stride, k_stride, v_stride;  // elements from token to token
     int n_seqs, total_q, total_k, n_heads, n_kv_heads, window;
     float scale;
+    int first_block;        // the blocks of launches before this one (set by the launcher)
 };
-int launch_attention_prefill(const AttentionPrefillArgs& a, int head_dim, hipStream_t stream);
+int launch_attention_prefill(AttentionPrefillArgs a, int head_dim, hipStream_t stream);
 
 // ---- logprobs.hip ------------------------------------------------------------------------------
 struct LogprobArgs {

@@ -113,9 +113,22 @@ int launch_rope_kv_write(const RopeKvArgs& a, bool bf16_rows, hipStream_t stream
     const int units = (a.n_heads + 2 * a.n_kv_heads) * (a.head_dim / 8);
     const int per_block = std::max(1, std::min(8, 512 / units));
     const size_t lds = (size_t)per_block * (a.rotary_dim / 2) * (a.k_scales ? sizeof(double2) : sizeof(float2));
+    const long long at_once = kMostThreads / 256 * per_block;
     auto run = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(a.n_tokens, per_block)), dim3(256), lds, stream, a, per_block);
-        return launch_status();
+        for (long long token = 0; token < a.n_tokens; token += at_once) {
+            RopeKvArgs b = a;
+            b.n_tokens = (int)std::min(a.n_tokens - token, at_once);
+            b.rows = static_cast<const char*>(a.rows) + token * a.stride * (bf16_rows ? 2 : 4);
+            if (a.positions) b.positions += token;
+            if (a.slots) b.slots += token;
+            if (a.q) b.q += token * a.n_heads * a.head_dim;
+            if (a.k) b.k += token * a.n_kv_heads * a.head_dim;
+            if (a.v) b.v += token * a.n_kv_heads * a.head_dim;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(b.n_tokens, per_block)), dim3(256), lds, stream, b, per_block);
+            const int rc = launch_status();
+            if (rc) return rc;
+        }
+        return (int)MOE_OK;
     };
     auto of_cache = [&](auto plain, auto mx) { return a.k_scales ? run(mx) : run(plain); };
     if (a.head_dim == 64)

@@ -76,7 +76,7 @@ def test_attention_prefill_refuses(pkg):
     assert all(call(**{name: None}) == -1 for name in ("out", "q", "k", "v", "qs", "ks"))
     assert all(call(**bad) == -2 for bad in (dict(n=0), dict(tq=0), dict(tk=0), dict(Hq=3), dict(D=72), dict(window=-1), dict(so=248), dict(sq=248), dict(sk=120),
                                              dict(sv=120), dict(so=260), dict(sk=132)))
-    assert call(n=65536) == call(tq=1 << 28) == call(Hq=1026, Hkv=2, so=1 << 20, sq=1 << 20) == call(sk=(1 << 24) + 8) == call(sv=(1 << 24) + 8) == -3
+    assert call(n=65536) == call(tq=1 << 28) == call(Hq=1026, Hkv=2, so=1 << 20, sq=1 << 20) == call(sk=(1 << 23) + 8) == call(sv=(1 << 23) + 8) == -3
     assert call(scale=0.0) == call(scale=float("nan")) == -5
     assert all(call(**bad) == -6 for bad in (dict(out=8), dict(q=8), dict(k=8), dict(v=8), dict(qs=2), dict(ks=2), dict(sinks=1)))
 
