@@ -44,7 +44,7 @@ MOE_DEVICE float mx_scale(uint32_t b) { return __uint_as_float(b == 255u ? 0x7FC
 // a query head into a lane column, so that its running maximum and sum are a lane's and P^T is the second product's operand as it stands: O^T = V^T P^T,
 // with V^T read as columns from LDS.  P goes into that product as two bf16 parts, to 2^-16 of a weight: the matrix units have time.  Statistics are
 // in powers of two: s' = scale log2(e) q.k.
-// Bound by HBM: 128 sequences of 4096 keys, 8 heads of 128 in 8 bits 178 us, 6.2 TB/s; one of 131072, 8 heads of 64, 44 us, 6.0 TB/s, and 4.7 for the join.
+// Bound by HBM: 128 sequences of 4096 keys, 8 heads of 128 in 8 bits 179 us, 6.2 TB/s; one of 131072, 8 heads of 64, 45 us, 6.0 TB/s, and 4.7 for the join.
 template <int D, bool MX>
 __global__ __launch_bounds__(64 * kWaves, 2) void attention_decode_kernel(AttentionDecodeArgs a) {
     constexpr int kRow = 2 * D, kSteps = D / 32, kDims = D / 16;

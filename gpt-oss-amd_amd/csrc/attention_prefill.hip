@@ -30,9 +30,9 @@ MOE_DEVICE Span span_of(const int* starts, int s, int total) {
 // it stands: O^T = V^T P^T, V^T read from LDS as columns.  P is rounded to bf16 for that product (half a step is up to 2^-8 of a weight, as that of the bf16
 // result; a second part would cost half as many matrix instructions again); its sum is taken before that, in fp32.  Statistics are in powers of two.
 // Longest blocks first.
-// A prompt of 8192, 64 heads of 64: 575 us, 957 TFLOP/s; heads of 128 1013; a large library product reaches 1394.  Without the weights' arithmetic it takes
-// 430 us, without matrix instructions 505.  64 rows to a wave, half the reads of LDS, and two or four blocks to a compute unit in place of three
-// change nothing (615 : 612 us at the time): what bounds it is what both kinds of instruction draw together.
+// A prompt of 8192, 64 heads of 64: 571 us, 963 TFLOP/s; heads of 128 990 to 1013; a large library product reaches 1394.  When it took 612 us, it took 439
+// without the weights' arithmetic and 505 without matrix instructions; 64 rows to a wave, half the reads of LDS, 615 : 618, two blocks to a compute unit
+// in place of three 613 : 612, four 784: what bounds it is both kinds of instruction together.
 template <int D>
 __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefill_kernel(AttentionPrefillArgs a) {
     constexpr int kRow = 2 * D, kSteps = D / 16, kDims = D / 32, kChunks = D / 8, kLoads = kKeys * kChunks / (64 * kWaves);
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     // whole rows to memory, by way of the wave's own part of LDS: in the order of the registers every store would touch 32 rows.  16 short-window prompts of
-    // up to 3000: 69 us : 62
+    // up to 3000: 70 us : 65
     uint8_t* rows = &lds[0][0][0] + wave * 32 * kRow;
 #pragma unroll
     for (int d = 0; d < kDims; ++d)
