@@ -54,15 +54,16 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
     if (!find_last_item(a.n_seqs, rank, tiles_of, seq, tile)) return;
     const Span qs = span_of(a.q_starts, seq, a.total_q), ks = span_of(a.k_starts, seq, a.total_k);
     const int ahead = ks.rows - qs.rows;  // query i sees keys up to i + ahead
+    const int window = a.window < ks.rows ? a.window : 0;  // one past all keys is none: a row without keys less such a window would not fit 32 bits
     const int row0 = tile * kRows, kv_head = head / (a.n_heads / a.n_kv_heads);
     const int end = min(row0 + kRows, qs.rows) + ahead;  // past the last key that the block sees
-    const int begin = a.window ? max(0, row0 + ahead - a.window + 1) & ~(kKeys - 1) : 0;
+    const int begin = window ? max(0, row0 + ahead - window + 1) & ~(kKeys - 1) : 0;
 
     __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][kKeys * kRow];
     __shared__ int odd[2];  // the first key of the last tile in that buffer whose values were not all finite
 
     const int wave_row = row0 + 32 * wave, row = min(wave_row + col, qs.rows - 1);
-    const int last = row + ahead, first = a.window ? last - a.window + 1 : 0;  // what this lane's row sees
+    const int last = row + ahead, first = window ? last - window + 1 : 0;  // what this lane's row sees
     u32x4 qf[kSteps];
     {
         const uint16_t* q = a.q + (size_t)(qs.begin + row) * a.q_stride + (size_t)head * D;
@@ -105,7 +106,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
     };
     // Whether some row of the block does not see all of these keys.  Infinities and NaNs among their values, which a weight of 0 does not undo, are taken
     // out of LDS in the careful pass; the rows that do see them get them afterwards.
-    auto cut = [&](int key0) { return key0 + kKeys - 1 > row0 + ahead || (a.window && key0 < end - a.window); };
+    auto cut = [&](int key0) { return key0 + kKeys - 1 > row0 + ahead || (window && key0 < end - window); };
     auto clean = [&](int buffer, int key0) {
         auto not_finite = [](uint32_t x) { return ((x & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((x & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u); };
 #pragma unroll
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
                 s[t] = mfma_32x32x16(*reinterpret_cast<const u32x4*>(k + r * kRow + k_chunk<D>(r, 2 * j + hi) * 16), qf[j], s[t]);
             }
         settle(s[0], s[1]);
-        if (key0 + kKeys - 1 > wave_row + ahead || (a.window && key0 < wave_row + 31 + ahead - a.window + 1)) {
+        if (key0 + kKeys - 1 > wave_row + ahead || (window && key0 < wave_row + 31 + ahead - window + 1)) {
             // a bit a key that the row sees, spread over its score; comparisons would each wait for the one before it to leave the condition register
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -226,7 +227,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
             if (key0 + kKeys < end) load(buffer ^ 1, key0 + kKeys);
             if (decltype(careful)::value && cut(key0)) clean(buffer, key0);
             // whether any row of the wave sees any of these keys
-            if (key0 <= wave_row + 31 + ahead && (!a.window || key0 + kKeys > wave_row + ahead - a.window + 1) && wave_row < qs.rows)
+            if (key0 <= wave_row + 31 + ahead && (!window || key0 + kKeys > wave_row + ahead - window + 1) && wave_row < qs.rows)
                 compute(buffer, key0, careful);
             buffer ^= 1;
         }
