@@ -696,6 +696,7 @@ int moe_attention_prefill(moe_bf16_t* out, const moe_bf16_t* q, const moe_bf16_t
     if ((out_stride | q_stride | k_stride | v_stride) % 8 != 0) return MOE_ERR_SHAPE;
     if (n_seqs > 65535 || (long long)total_q * n_heads >= (1 << 30)) return MOE_ERR_LIMIT;
     if (std::max(k_stride, v_stride) > (1 << 23)) return MOE_ERR_LIMIT;  // 64 rows within 31 bits of bytes
+    if (total_k > kMostRows) return MOE_ERR_LIMIT;  // keys are counted up to whole tiles
     if (bad_scale(scale)) return MOE_ERR_FORMAT;
     if (misaligned({out, q, k, v}, 16) || misaligned({q_starts, k_starts}, 4) || misaligned({sinks}, 2)) return MOE_ERR_ALIGN;
     return launch_attention_prefill({out, q, k, v, q_starts, k_starts, sinks, out_stride, q_stride, k_stride, v_stride, n_seqs, total_q, total_k, n_heads,

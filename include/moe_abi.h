@@ -384,8 +384,8 @@ MOE_API int moe_attention_decode(moe_bf16_t* out, const moe_bf16_t* q, const moe
  * a window, j > i + m - n - window.  The rest as moe_attention_decode, with weights rounded to bf16.  Rows that belong to no sequence are not written.  What one row
  * sees does not depend on keys that it does not see, whatever these and their values hold; a row's result does not depend on other sequences.
  * q, out [total_q, n_heads, head_dim], k, v [total_k, n_kv_heads, head_dim] bf16, *_stride elements from token to token (at least a token's, a
- * multiple of 8; k_stride, v_stride <= 2^23); starts ascending (what lies outside the rows is cut off).  head_dim 64 or 128; n_seqs <= 65535; total_q * n_heads < 2^30; all
- * tensors 16-byte aligned, starts 4-byte. */
+ * multiple of 8; k_stride, v_stride <= 2^23); starts ascending (what lies outside the rows is cut off).  head_dim 64 or 128; n_seqs <= 65535; total_q * n_heads < 2^30;
+ * total_k < 2^31 - 255; all tensors 16-byte aligned, starts 4-byte. */
 MOE_API int moe_attention_prefill(moe_bf16_t* out, const moe_bf16_t* q, const moe_bf16_t* k, const moe_bf16_t* v, const int* q_starts,
                                   const int* k_starts, int n_seqs, int total_q, int total_k, int n_heads, int n_kv_heads, int head_dim,
                                   long long out_stride, long long q_stride, long long k_stride, long long v_stride, int window, float scale,
