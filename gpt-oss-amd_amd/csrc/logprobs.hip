@@ -381,7 +381,7 @@ __global__ __launch_bounds__(64 * kWaves) void logprob_join_kernel(LogprobArgs a
 // 1000 rows of 131072 90 : 99 : 111, 100 rows 33 : 34 : 37.
 constexpr int kBlocks = 512;
 static int parts_of(int n_tokens, int vocab) {
-    return std::min(ceil_div(kBlocks, n_tokens), ceil_div(vocab, kFewest));
+    return n_tokens >= kBlocks ? 1 : std::min(ceil_div(kBlocks, n_tokens), ceil_div(vocab, kFewest));
 }
 
 size_t logprob_workspace(int n_tokens, int vocab, int top_k) {
@@ -394,14 +394,14 @@ size_t logprob_workspace(int n_tokens, int vocab, int top_k) {
 int launch_token_logprobs(const LogprobArgs& a, bool bf16_logits, hipStream_t stream) {
     const int parts = parts_of(a.n_tokens, a.vocab), part_len = ceil_div(ceil_div(a.vocab, parts), kStep) * kStep;
     auto run = [&](auto kernel, auto join) {
-        const int most = (int)(kMostThreads / (64 * kWaves));  // rows of a launch; more than 1024 of them are not cut
-        for (int row = 0; row < a.n_tokens; row += most) {
+        const long long most = kMostThreads / (64 * kWaves);  // rows of a launch; more than 1024 of them are not cut
+        for (long long row = 0; row < a.n_tokens; row += most) {
             LogprobArgs b = a;
-            b.n_tokens = std::min(a.n_tokens - row, most);
-            b.logits = static_cast<const char*>(a.logits) + (size_t)row * a.stride * (bf16_logits ? 2 : 4);
+            b.n_tokens = (int)std::min(a.n_tokens - row, most);
+            b.logits = static_cast<const char*>(a.logits) + row * a.stride * (bf16_logits ? 2 : 4);
             if (a.logprobs) b.tokens += row, b.logprobs += row;
             if (a.entropy) b.entropy += row;
-            if (a.top_k) b.top_logprobs += (size_t)row * a.top_k, b.top_indices += (size_t)row * a.top_k;
+            if (a.top_k) b.top_logprobs += row * a.top_k, b.top_indices += row * a.top_k;
             hipLaunchKernelGGL(kernel, dim3((unsigned)(b.n_tokens * parts)), dim3(64 * kWaves), 0, stream, b, parts, part_len);
             const int rc = launch_status();
             if (rc) return rc;
