@@ -15,6 +15,11 @@ constexpr int kWaves = 4, kRows = 32 * kWaves, kKeys = 64;  // query rows of a b
 // has to look for one, and with weights up to 2^10 sums stay as far from overflow as values of 2^118 allow.
 constexpr float kMostWeight = 1024.f;
 
+// A weight is exp2 of s scale - m in one rounding, the maximum m a product that was rounded by itself: what it lost, up to 2^-24 of m, is a factor of all weights
+// of the row, which their sum takes out again.  Up to this size of m it is below 2^(1/16); from 2^31 on it would be infinity or nothing.  Rows whose
+// maximum was ever past it go through the careful pass with scores rounded before the maximum is taken.
+constexpr float kFar = 1048576.f;
+
 struct Span {
     int begin, rows;
 };
@@ -75,8 +80,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
     for (int d = 0; d < kDims; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, reach = 0.f;  // reach: the largest |m| so far
     const float scale = a.scale * kLog2e;
+    float before = 1.f, by = scale;  // of the careful pass: what scores are multiplied by first, and next to the maximum
 
     // a lane's share of a tile: kLoads pieces of 1 KiB to a wave, each linear in LDS; offsets in bytes from the tile's first row, of rows past the last key
     // the last one's
@@ -157,6 +163,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
                 }
             }
         }
+        if constexpr (decltype(careful)::value) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[0][i] *= before;
+                s[1][i] *= before;
+            }
+        }
+        const float factor = decltype(careful)::value ? by : scale;
         u32x4 p[4];
         auto weigh = [&](float base) {
             float sum[2] = {0.f, 0.f};
@@ -164,7 +178,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[t][i], scale, -base)), y = __builtin_amdgcn_exp2f(fmaf(s[t][i + 1], scale, -base));
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[t][i], factor, -base)), y = __builtin_amdgcn_exp2f(fmaf(s[t][i + 1], factor, -base));
                     sum[0] += x;
                     sum[1] += y;
                     p[2 * t + i / 8][i % 8 / 2] = pack_bf16x2(x, y);
@@ -178,9 +192,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) most = fmaxf(most, s[t][i]);
-            most = max_of_halves(sum < kMostWeight ? 0.f : 1.f) > 0.f ? fmaxf(m, max_of_halves(most) * scale) : m;  // of the rows that have to
+            most = max_of_halves(sum < kMostWeight ? 0.f : 1.f) > 0.f ? fmaxf(m, max_of_halves(most) * factor) : m;  // of the rows that have to
             const float down = most == m ? 1.f : __builtin_amdgcn_exp2f(m - most);
             m = most;
+            if (m > -INFINITY) reach = fmaxf(reach, fabsf(m));
             l *= down;
 #pragma unroll
             for (int d = 0; d < kDims; ++d) acc[d] *= down;
@@ -242,13 +257,18 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void attention_prefil
         for (int d = 0; d < kDims; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sum = fmaf(acc[d][i], 0.f, sum);  // 0 if all are finite
-        if (__syncthreads_or(!(sum == 0.f))) {
+        const bool far = reach > kFar;
+        if (__syncthreads_or(!(sum == 0.f) || far)) {
 #pragma unroll
             for (int d = 0; d < kDims; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
             m = -INFINITY;
             l = 0.f;
+            if (far) {
+                before = scale;
+                by = 1.f;
+            }
             if (threadIdx.x < 2) odd[threadIdx.x] = -1;
             offsets(kKeys);
             pass(std::true_type{});
