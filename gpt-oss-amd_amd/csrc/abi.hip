@@ -624,7 +624,7 @@ static int check_cache(const moe_kv_cache* c) {
     return misaligned({c->k, c->v}, 16) ? MOE_ERR_ALIGN : MOE_OK;
 }
 static inline int log2_of(int power) { return __builtin_ctz((unsigned)power); }
-static inline bool bad_scale(float scale) { return !(scale > 0.f) || scale > 3.4028234e38f; }
+static inline bool bad_scale(float scale) { return !(scale > 0.f) || scale > 1.7014118e38f; }  // up to 2^127: the kernels take it times log2(e)
 
 int moe_rope_kv_write(const void* qkv, int qkv_type, long long stride, const int* positions, const float* inv_freq, int n_tokens, int n_heads,
                       int n_kv_heads, int head_dim, int rotary_dim, float scale, moe_bf16_t* q, moe_bf16_t* k, moe_bf16_t* v,

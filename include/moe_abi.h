@@ -371,7 +371,7 @@ MOE_API int moe_rope_kv_write(const void* qkv, int qkv_type, long long stride, c
  * A page number outside [0, n_pages) is a page without keys, and page numbers behind a sequence's last key are not looked at: a table may hold
  * anything there, as may the slots.  Deterministic, but the sum over keys is cut into pieces that depend on all the lengths of a call.
  * q, out [batch, n_heads, head_dim] bf16, page_table [batch, max_pages], lengths [batch], sinks [n_heads] bf16 or NULL.  n_heads <= 1024, a multiple of
- * n_kv_heads; scale > 0 and finite; batch <= 65535; max_pages * page_size <= 2^30; q and out 16-byte aligned.  workspace:
+ * n_kv_heads; scale > 0 and <= 2^127; batch <= 65535; max_pages * page_size <= 2^30; q and out 16-byte aligned.  workspace:
  * moe_attention_decode_workspace_bytes (0 for sizes that the call rejects; a batch's serves smaller ones), 16-byte aligned; its content
  * does not matter.  Calls that overlap in time need workspaces of their own.  out may not overlap an input. */
 MOE_API size_t moe_attention_decode_workspace_bytes(int batch, int n_heads, int n_kv_heads, int head_dim);
