@@ -367,7 +367,9 @@ MOE_API int moe_rope_kv_write(const void* qkv, int qkv_type, long long stride, c
  * Query heads g, g + 1, .. share a key/value head: head h reads key/value head h / (n_heads / n_kv_heads).
  *   s[j] = scale q . k[j],  out = sum_j exp(s[j]) v[j] / (sum_j exp(s[j]) + exp(sinks[h]))    (without sinks: without their term)
  * A query that sees nothing has zeros.  Products of bf16 values, sums and statistics in fp32, weights exp(s) to 2^-16; the result is rounded once.
- * What is not finite among the keys and values that a query sees makes NaNs or infinities of its results.
+ * Sums are divided at the end: the keys that a query sees, as many as they are, times the largest |value| among them have to stay below 2^127.
+ * What is not finite among the keys and values that a query sees makes NaNs or infinities of its results, but for a score of -infinity, which has no
+ * weight.  A sink of -infinity is none; one of +infinity or a NaN makes NaNs.
  * A page number outside [0, n_pages) is a page without keys, and page numbers behind a sequence's last key are not looked at: a table may hold
  * anything there, as may the slots.  Deterministic, but the sum over keys is cut into pieces that depend on all the lengths of a call.
  * q, out [batch, n_heads, head_dim] bf16, page_table [batch, max_pages], lengths [batch], sinks [n_heads] bf16 or NULL.  n_heads <= 1024, a multiple of
@@ -381,8 +383,9 @@ MOE_API int moe_attention_decode(moe_bf16_t* out, const moe_bf16_t* q, const moe
 
 /* Causal attention over prompts packed one after another: sequence s has the query rows q_starts[s] .. q_starts[s + 1] - 1 of total_q and the key and value
  * rows k_starts[s] .. k_starts[s + 1] - 1 of total_k.  Its queries are its last positions: query i of n sees key j of m if j <= i + m - n and, with
- * a window, j > i + m - n - window.  The rest as moe_attention_decode, with weights rounded to bf16.  Rows that belong to no sequence are not written.  What one row
- * sees does not depend on keys that it does not see, whatever these and their values hold; a row's result does not depend on other sequences.
+ * a window, j > i + m - n - window.  The rest as moe_attention_decode, with weights rounded to bf16 and relative to a maximum that may be 2^10 behind: keys times
+ * the largest |value| have to stay below 2^115.  Rows that belong to no sequence are not written.  What one row sees does not depend on keys that it
+ * does not see, whatever these and their values hold; a row's result does not depend on other sequences.
  * q, out [total_q, n_heads, head_dim], k, v [total_k, n_kv_heads, head_dim] bf16, *_stride elements from token to token (at least a token's, a
  * multiple of 8; k_stride, v_stride <= 2^23); starts ascending (what lies outside the rows is cut off).  head_dim 64 or 128; n_seqs <= 65535; total_q * n_heads < 2^30;
  * total_k < 2^31 - 255; all tensors 16-byte aligned, starts 4-byte. */
