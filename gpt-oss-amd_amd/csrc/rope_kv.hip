@@ -8,10 +8,18 @@
 
 namespace moe {
 
+// p f / (2 pi) less the nearest whole number, to 2^-53: the product (31 by 24 bits) and 1 / (2 pi) as two numbers each, and what the product of the leading two
+// leaves.  One rounding of each alone is off by 2^-21 of the angle's cosine at positions next to 2^31, and by codes of the 8-bit cache from far fewer on.
+MOE_DEVICE double part_of_turn(double p, double f) {
+#pragma clang fp contract(off)  // a product fused with the difference would have its rest taken twice
+    constexpr double c = 0x1.45f306dc9c883p-3, c_rest = -0x1.6b01ec5417056p-57;
+    const double angle = p * f, angle_rest = fma(p, f, -angle), turns = angle * c;
+    return (turns - rint(turns)) + (fma(angle, c, -turns) + fma(angle_rest, c, angle * c_rest));
+}
+
 // Pairs (u, v) = (x[i], x[i + rotary_dim / 2]) of a head turn by the angle p inv_freq[i]: (u cos - v sin, v cos + u sin), times a.scale; the
 // rest of a head stays.  A thread takes four pairs, so that what it holds lies in two runs of four values, eight lanes to 32 values: the groups of
-// the 8-bit cache.  The angle is taken in turns in fp64 (2^-53 of it: 31 bits of position by 24 of frequency), of which the fraction alone
-// goes to fp32; cosines and sines are made once a token, in LDS.  Keys for an 8-bit cache turn in fp64 and are rounded once, so that a key next to the
+// the 8-bit cache.  The angle is taken in turns, of which the fraction alone goes to fp32; cosines and sines are made once a token, in LDS.  Keys for an 8-bit cache turn in fp64 and are rounded once, so that a key next to the
 // middle of two codes goes where the formula puts it.  Bound by HBM: 20 KiB in and 13 out for a token of 64 + 2 * 8 heads of 64; 8192 of them with packed
 // rows 51 us, 5.3 TB/s, what a copy reaches.
 template <int D, bool BF16, bool MX>
@@ -22,10 +30,10 @@ __global__ __launch_bounds__(256) void rope_kv_kernel(RopeKvArgs a, int tokens_p
     const int R = a.rotary_dim, half = R / 2;
     const int token0 = blockIdx.x * tokens_per_block, tokens = min(tokens_per_block, a.n_tokens - token0);
     for (int i = threadIdx.x; i < tokens * half; i += 256) {
-        const double turns = (double)a.positions[token0 + i / half] * (double)a.inv_freq[i % half] * 0.15915494309189533577;
+        const double turns = part_of_turn((double)a.positions[token0 + i / half], (double)a.inv_freq[i % half]);
         decltype(Turn::x) sine, cosine;
-        if constexpr (MX) sincospi(2.0 * (turns - rint(turns)), &sine, &cosine);
-        else sincospif(2.f * (float)(turns - rint(turns)), &sine, &cosine);
+        if constexpr (MX) sincospi(2.0 * turns, &sine, &cosine);
+        else sincospif(2.f * (float)turns, &sine, &cosine);
         turn[i].x = cosine * a.scale;
         turn[i].y = sine * a.scale;
     }

@@ -348,7 +348,7 @@ typedef struct moe_kv_cache {
 
 /* Rotary embedding and cache write.  qkv holds n_tokens rows, `stride` elements apart, of n_heads queries, n_kv_heads keys and n_kv_heads values of
  * head_dim each, fp32 or bf16 (qkv_type MOE_ROWS_*).  Of every query and key the first rotary_dim values turn: with p = positions[token],
- * i < rotary_dim / 2, a = p * inv_freq[i] (exact, in fp64), u = x[i], v = x[i + rotary_dim / 2]:
+ * i < rotary_dim / 2, a = p * inv_freq[i] (exact for |a| < 2^50), u = x[i], v = x[i + rotary_dim / 2]:
  *   x[i] = scale (u cos a - v sin a),  x[i + rotary_dim / 2] = scale (v cos a + u sin a)   in fp32, cos and sin to 2^-22; in fp64 for an 8-bit cache
  * Then what is asked for, at least one:
  *   q, k, v   [n_tokens, n_heads or n_kv_heads, head_dim] bf16, each or NULL (k and v for moe_attention_prefill)
