@@ -577,7 +577,7 @@ def attention_decode(out, q, cache, page_table, lengths, batch, n_heads, scale, 
     rc = _lib.moe_attention_decode(_arg("out", out, _bf16, n, dev), _arg("q", q, _bf16, n, dev), cache.of(dev),
                                    _arg("page_table", page_table, torch.int32, batch * max_pages, dev), _arg("lengths", lengths, torch.int32, batch, dev),
                                    batch, n_heads, max_pages, window, scale, _arg("sinks", sinks, _bf16, n_heads, dev),
-                                   _arg("workspace", workspace, _u8, 0, dev), workspace.numel(), _stream(stream, dev))
+                                   _arg("workspace", workspace, _u8, 0, dev), 0 if workspace is None else workspace.numel(), _stream(stream, dev))
     if rc:
         raise MoeError("moe_attention_decode", rc)
 

@@ -15,3 +15,16 @@ def test_scales_that_log2_e_takes_past_fp32_are_refused(pkg):
     for call in (prefill, decode):
         assert call(1.8e38) == call(3.4e38) == -5
         assert call(2.0 ** 127) == call(1e-45) == -6  # past the scale's check: the sinks' address stops them
+
+
+def test_a_missing_workspace_is_the_library_s_error(pkg, monkeypatch):
+    import pytest
+    import torch
+    monkeypatch.setattr(pkg, "_device", lambda: -1)  # host tensors pass for the current device's: the call ends before it reads them
+    z = torch.zeros
+    cache = pkg.KvCache(z(4, 2, 16, 64).bfloat16(), z(4, 2, 16, 64).bfloat16())
+    q, i = z(2, 4, 64).bfloat16(), z(2, 4, dtype=torch.int32)
+    with pytest.raises(pkg.MoeError):
+        pkg.attention_decode(q, q, cache, i, i[0], 2, 4, 1.0, None, stream=0)
+    with pytest.raises(pkg.MoeError):
+        pkg.token_logprobs(z(2, 5000), i, 2, 5000, logprobs=z(2), stream=0)
