@@ -309,8 +309,8 @@ MOE_DEVICE void write_row(const LogprobArgs& a, int row, float token, const Sums
 // maximum is the wave's, so that most steps change neither it nor the list of the largest values, which is what one comparison of each lane's
 // largest value asks, and cost a difference, an exponential and two sums a value.  Values before the first 16-byte border and behind the
 // last whole step are read one by one, by the last wave while its first steps come.  Past the last-level cache rows are read past it.
-// Bound by HBM and by its arithmetic: 1000 bf16 rows of 200000 with 5 alternatives 78 to 83 us, 5 TB/s (without the entropy 75, without any sums 70); fp32
-// rows of 131072 with 20 89 us, 5.9 TB/s.  One row of 131072 with 20 alternatives 10.8 us, 5.9 and 4.9 of them the two launches.
+// Bound by HBM and by its arithmetic: 1000 bf16 rows of 200000 with 5 alternatives 79 to 90 us, 4.4 to 5.1 TB/s (when it took 83: without the entropy 75, without any
+// sums 70); fp32 rows of 131072 with 20 87 us, 6 TB/s.  One row of 131072 with 20 alternatives 11.0 us, 6.1 and 4.9 of them the two launches.
 template <class T, bool NT>
 __global__ __launch_bounds__(64 * kWaves) void logprob_kernel(LogprobArgs a, int parts, int part_len) {
     constexpr int kVec = 16 / sizeof(T);  // values of a load
